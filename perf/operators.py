@@ -27,29 +27,29 @@ def listed():
     teach = dict(op="distill", masked=False)
     return [
         # training of a layer of ordinary width in the half-wide type: 4 sequences of 2048 positions
-        dict(conv, name="convolution, train", mode="train", type="bf16", batch=4, time=2048, width=4096),
+        dict(conv, name="convolution train", mode="train", type="bf16", batch=4, time=2048, width=4096),
         # 64 sequences answered token by token: one new position each, the last three inputs kept
-        dict(conv, name="convolution, tokens", mode="token", type="f32", batch=64, time=1, width=2048),
+        dict(conv, name="convolution tokens", mode="token", type="f32", batch=64, time=1, width=2048),
         # one long prompt alone: few channels, many positions, so the length has to give the parallel work
-        dict(scan, name="scan, long prompt", mode="prompt", type="bf16", batch=1, time=4096, width=4096, states=16, state=False),
+        dict(scan, name="scan long prompt", mode="prompt", type="bf16", batch=1, time=4096, width=4096, states=16, state=False),
         # a training step on 8 sequences
-        dict(scan, name="scan, train", mode="train", type="bf16", batch=8, time=1024, width=2048, states=16),
+        dict(scan, name="scan train", mode="train", type="bf16", batch=8, time=1024, width=2048, states=16),
         # the width of the ragged regression network, sequences of different lengths, a number of states that divides by nothing
-        dict(scan, name="scan, ragged train", mode="train", type="f32", batch=7, time=203, width=333, states=7, groups=3, gate=False, ragged=True),
+        dict(scan, name="scan ragged train", mode="train", type="f32", batch=7, time=203, width=333, states=7, groups=3, gate=False, ragged=True),
         # 256 sequences answered token by token: bound by their states
-        dict(scan, name="scan, tokens", mode="token", type="bf16", batch=256, time=1, width=4096, states=16),
+        dict(scan, name="scan tokens", mode="token", type="bf16", batch=256, time=1, width=4096, states=16),
         # a single sequence answered token by token: only latency counts
-        dict(scan, name="scan, one token", mode="token", type="f32", batch=1, time=1, width=1024, states=16),
+        dict(scan, name="scan one token", mode="token", type="f32", batch=1, time=1, width=1024, states=16),
         # a classifier of 1024 outputs taught by a larger one, labels mixed in: the batch of the wide network
-        dict(teach, name="distill, classes", type="f32", rows=4096, vocabulary=1024, top=16, temperature=2.0, hard=0.5),
+        dict(teach, name="distill classes", type="f32", rows=4096, vocabulary=1024, top=16, temperature=2.0, hard=0.5),
         # 2048 positions of a large vocabulary, the teacher's 64 best logits stored for each
-        dict(teach, name="distill, large vocabulary", type="bf16", rows=2048, vocabulary=131072, top=64, temperature=1.0, hard=0.0),
+        dict(teach, name="distill large vocabulary", type="bf16", rows=2048, vocabulary=131072, top=64, temperature=1.0, hard=0.0),
         # a padded batch of few positions: rows without weight, lists that end early, a vocabulary off every boundary
-        dict(teach, name="distill, ragged", type="f16", rows=203, vocabulary=32001, top=50, temperature=1.5, hard=0.25, masked=True),
+        dict(teach, name="distill ragged", type="f16", rows=203, vocabulary=32001, top=50, temperature=1.5, hard=0.25, masked=True),
         # one row: a single sequence that waits for its next token
-        dict(op="sample", name="sample, one row", type="f32", rows=1, vocabulary=32000, settings="one", masked=False),
+        dict(op="sample", name="sample one row", type="f32", rows=1, vocabulary=32000, settings="one", masked=False),
         # 256 sequences of a large vocabulary, each with settings of its own
-        dict(op="sample", name="sample, batch", type="bf16", rows=256, vocabulary=131072, settings="mixed", masked=False),
+        dict(op="sample", name="sample batch", type="bf16", rows=256, vocabulary=131072, settings="mixed", masked=False),
     ]
 
 
