@@ -373,6 +373,86 @@ int myea_b200_gemm_nt(int device, int engine, uint64_t M, uint64_t N, uint64_t K
 int myea_b200_gemm_nt_static(int device, uint64_t M, uint64_t N, uint64_t K, const float *device_A, const float *device_B,
                              float *device_C, int accumulate, void *stream, char *error_message, size_t error_capacity);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Operators for sequence models, beside the recurrent layers, the output error and the output layer above.  No counterpart
+ * in the reference.  They need no handle: every array is DEVICE memory of the caller on GPU `device`, calls are asynchronous
+ * on `stream` (a cudaStream_t, null: the default stream), may be captured into a CUDA graph, allocate nothing and leave the
+ * caller's current device as it was.  Working memory is the caller's too: a *_workspace function says how many bytes a call
+ * with these sizes takes (256-byte aligned; 0: none), and calls that may overlap on the GPU take one each.  Sums run in a
+ * fixed order: the same call gives the same bits.  On a status other than MYEA_OK nothing was launched (MYEA_E_CUDA: perhaps
+ * a part) and error_message (optional, error_capacity bytes) says why.  Outputs overlap neither inputs nor each other except
+ * where that is said.
+ *
+ * Activations and their errors are of one type (MYEA_TYPE_*) per call; parameters, their derivatives, states of a scan and
+ * losses are fp32, and so is all arithmetic.  A myea_view is a [batch][time][...] array whose last dimensions lie densely:
+ * element (b, t, c) at data[b * stride_batch + t * stride_time + c], strides in elements, so that batch-major and time-major
+ * arrays and slices of wider ones are all read and written where they lie.
+ * `lengths` (int32[batch], may be null: all `time`): positions of a sequence from its length on are not read, and written as
+ * 0 in outputs and errors; values outside 0..time count as the nearest of the two.  `accumulate`: parameter derivatives are
+ * added to what their arrays hold, as in the sub-batches of a mini-batch; otherwise they replace it. */
+#define MYEA_TYPE_F32 0u
+#define MYEA_TYPE_BF16 1u
+#define MYEA_TYPE_F16 2u
+
+typedef struct myea_view {
+  void *data;
+  int64_t stride_batch, stride_time;
+} myea_view;
+
+/* Short causal convolution over time, one filter per channel:  a = bias[c] + sum over j < taps of weight[c][j] *
+ * x[t - taps + 1 + j][c],  y = a * sigmoid(a) (silu = 1) or a.  Inputs before the first position come from `state`
+ * [batch][taps - 1][width] (null: zeros), the last taps - 1 inputs of every sequence leave in `final_state` (may be null, may
+ * be `state`); a single token is time = 1 with both.  1 <= taps <= 8.
+ * Backward (reads x, weight, bias, state, dy; d_final_state may be null): dx, d_weight [width][taps], d_bias [width],
+ * d_state [batch][taps - 1][width], each of which may be null. */
+typedef struct myea_convolution {
+  uint32_t type, taps, silu, accumulate;
+  uint64_t batch, time, width;
+  myea_view x, y, dy, dx;
+  const float *weight, *bias;
+  const void *state;
+  void *final_state;
+  const int32_t *lengths;
+  float *d_weight, *d_bias;
+  const void *d_final_state;
+  void *d_state;
+} myea_convolution;
+int myea_b200_causal_convolution(int device, const myea_convolution *c, void *stream, char *error_message, size_t error_capacity);
+size_t myea_b200_causal_convolution_backward_workspace(const myea_convolution *c);
+int myea_b200_causal_convolution_backward(int device, const myea_convolution *c, void *workspace, size_t workspace_bytes, void *stream,
+                                          char *error_message, size_t error_capacity);
+
+/* Selective state space scan.  Channel c of group g = c / (width / groups) carries `states` values:
+ *   s = delta[t][c] + delta_bias[c], through log(1 + e^s) where softplus = 1
+ *   h[n] <- exp(s * A[c][n]) * h[n] + s * u[t][c] * B[t][g][n]        y[t][c] = sum over n of C[t][g][n] * h[n] + D[c] * u[t][c]
+ * and y is multiplied by z * sigmoid(z) where z is given.  u, delta, z, y: [batch][time][width]; B, C: [batch][time][groups *
+ * states]; A [width][states]; D, delta_bias [width] (may be null); state, final_state [batch][width][states] (may be null: zeros /
+ * not wanted; may be the same array).  A single token is time = 1 with both.  1 <= states <= 128, groups divides width.
+ * For training the forward pass leaves the state before every 16th position in `checkpoints` (null: no backward pass follows).
+ * Backward (reads all inputs, checkpoints and dy; d_final_state may be null): du, ddelta, dB, dC, dz (null where z is), d_A,
+ * d_D, d_delta_bias (null where D / delta_bias is), d_state (may be null). */
+typedef struct myea_scan {
+  uint32_t type, softplus, accumulate, reserved;
+  uint64_t batch, time, width, states, groups;
+  myea_view u, delta, B, C, z, y;
+  const float *A, *D, *delta_bias;
+  const float *state;
+  float *final_state;
+  const int32_t *lengths;
+  float *checkpoints;
+  myea_view dy, du, ddelta, dB, dC, dz;
+  float *d_A, *d_D, *d_delta_bias;
+  const float *d_final_state;
+  float *d_state;
+} myea_scan;
+size_t myea_b200_selective_scan_checkpoint_bytes(const myea_scan *s);
+size_t myea_b200_selective_scan_workspace(const myea_scan *s);
+int myea_b200_selective_scan(int device, const myea_scan *s, void *workspace, size_t workspace_bytes, void *stream, char *error_message,
+                             size_t error_capacity);
+size_t myea_b200_selective_scan_backward_workspace(const myea_scan *s);
+int myea_b200_selective_scan_backward(int device, const myea_scan *s, void *workspace, size_t workspace_bytes, void *stream, char *error_message,
+                                      size_t error_capacity);
+
 /* Per-kernel-class device time of the handle since the last call with reset!=0 (CUDA events on the handle's
  * stream); classes: 0 gemm, 1 split/pack, 2 normalization, 3 elementwise, 4 optimizer, 5 recurrent cell. */
 #define MYEA_TIMER_CLASSES 8

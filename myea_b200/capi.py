@@ -62,6 +62,28 @@ class OptDesc(C.Structure):
                 ("regularization__l1", C.c_float), ("regularization__l2", C.c_float)]
 
 
+# operators for sequence models
+TYPE_F32, TYPE_BF16, TYPE_F16 = range(3)
+
+
+def _views(*names):
+    """myea_view members: address, strides over batch and time"""
+    return [(n + tail, t) for n in names for tail, t in (("", C.c_void_p), ("_batch", C.c_int64), ("_time", C.c_int64))]
+
+
+class Convolution(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("type", "taps", "silu", "accumulate")] + [(n, C.c_uint64) for n in ("batch", "time", "width")] +
+                _views("x", "y", "dy", "dx") +
+                [(n, C.c_void_p) for n in ("weight", "bias", "state", "final_state", "lengths", "d_weight", "d_bias", "d_final_state", "d_state")])
+
+
+class Scan(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("type", "softplus", "accumulate", "reserved")] +
+                [(n, C.c_uint64) for n in ("batch", "time", "width", "states", "groups")] + _views("u", "delta", "B", "C", "z", "y") +
+                [(n, C.c_void_p) for n in ("A", "D", "delta_bias", "state", "final_state", "lengths", "checkpoints")] +
+                _views("dy", "du", "ddelta", "dB", "dC", "dz") + [(n, C.c_void_p) for n in ("d_A", "d_D", "d_delta_bias", "d_final_state", "d_state")])
+
+
 class LayerIndex(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in
                 ("first_connection_index", "last_connection_index", "first_bias_connection_index",
@@ -222,6 +244,14 @@ _PROTOS = {
                                     C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c_int]),
     "myea_b200_gemm_nt_static": (C.c_int, [C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p,
                                            C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_causal_convolution": (C.c_int, [C.c_int, C.POINTER(Convolution), C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_causal_convolution_backward_workspace": (C.c_size_t, [C.POINTER(Convolution)]),
+    "myea_b200_causal_convolution_backward": (C.c_int, [C.c_int, C.POINTER(Convolution), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_selective_scan_checkpoint_bytes": (C.c_size_t, [C.POINTER(Scan)]),
+    "myea_b200_selective_scan_workspace": (C.c_size_t, [C.POINTER(Scan)]),
+    "myea_b200_selective_scan": (C.c_int, [C.c_int, C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_selective_scan_backward_workspace": (C.c_size_t, [C.POINTER(Scan)]),
+    "myea_b200_selective_scan_backward": (C.c_int, [C.c_int, C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
     "myea_b200_profile": (C.c_int, [C.c_void_p, C.c_int]),
     "myea_b200_profile_read": (C.c_int, [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_uint64),
                                          C.POINTER(C.c_double), C.c_int]),
