@@ -453,6 +453,55 @@ size_t myea_b200_selective_scan_backward_workspace(const myea_scan *s);
 int myea_b200_selective_scan_backward(int device, const myea_scan *s, void *workspace, size_t workspace_bytes, void *stream, char *error_message,
                                       size_t error_capacity);
 
+/* Error against a teacher's best logits, beside the output error of a network.  The teacher gives `top` (index, logit) pairs per
+ * row, in any order; an index outside 0..vocabulary-1 is an entry that is not there, entries of one index add up.  With p the softmax of
+ * the row's teacher logits over temperature, q the softmax of `logits` over temperature and r the softmax of `logits`:
+ *   losses[row] = weight[row] * (soft * temperature^2 * sum over entries of p * (log p - log q[index]) - hard * log r[label])
+ * d_logits (null: only the losses; may be `logits`): the derivatives of losses[row] with respect to the row's logits, of their type.  A
+ * row without entries has no soft term, a label outside the vocabulary (or labels = null) no hard term, and a row of weight 0 is not
+ * read: loss and derivatives are 0.  Logits of minus infinity are closed words; a row without an open one has no softmax and counts
+ * as one of weight 0.  Rows are stride elements apart.  1 <= top <= 1024,
+ * temperature > 0. */
+typedef struct myea_distillation {
+  uint32_t type, reserved;
+  uint64_t rows, vocabulary, top;
+  const void *logits;
+  int64_t logits_stride;
+  const int32_t *index;
+  int64_t index_stride;
+  const float *teacher;
+  int64_t teacher_stride;
+  const int32_t *labels;
+  const float *weight;
+  float temperature, soft, hard, reserved2;
+  float *losses;
+  void *d_logits;
+  int64_t d_logits_stride;
+} myea_distillation;
+int myea_b200_distillation_error(int device, const myea_distillation *d, void *stream, char *error_message, size_t error_capacity);
+
+/* One token for every row of `logits`, drawn with the given random number (uniform[row] in [0, 1)), beside the output layer's
+ * values.  With m the row's largest logit, w[i] = exp((logits[i] - m) / temperature[row]), tokens ordered by falling logit and, where
+ * these are equal, rising index:  top_k > 0 keeps the first top_k;  top_p < 1 keeps of these every token before which less than
+ * top_p of their sum of w lies, and the first in any case;  min_p > 0 keeps what has w >= min_p.  The draw goes through the kept tokens by rising
+ * index: the first whose running sum of w exceeds uniform * (their sum).  temperature <= 0: the largest logit, the lowest index where several
+ * are.  Settings are arrays of one value per row; null: temperature 1, no limit.  Minus infinity and NaN are closed words; a row
+ * without any other has token -1 and chance 0.  Words of plus infinity share the draw alone.  chances (may be null): w / sum of the token.
+ * Weights are summed as integers of 62 bits less those that count the vocabulary, so that the draw is that of exact sums up to 1e-12
+ * and does not depend on the order of summation. */
+typedef struct myea_sampling {
+  uint32_t type, reserved;
+  uint64_t rows, vocabulary;
+  const void *logits;
+  int64_t logits_stride;
+  const float *uniform, *temperature;
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+  int32_t *tokens;
+  float *chances;
+} myea_sampling;
+int myea_b200_sample(int device, const myea_sampling *s, void *stream, char *error_message, size_t error_capacity);
+
 /* Per-kernel-class device time of the handle since the last call with reset!=0 (CUDA events on the handle's
  * stream); classes: 0 gemm, 1 split/pack, 2 normalization, 3 elementwise, 4 optimizer, 5 recurrent cell. */
 #define MYEA_TIMER_CLASSES 8

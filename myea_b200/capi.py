@@ -84,6 +84,19 @@ class Scan(C.Structure):
                 _views("dy", "du", "ddelta", "dB", "dC", "dz") + [(n, C.c_void_p) for n in ("d_A", "d_D", "d_delta_bias", "d_final_state", "d_state")])
 
 
+class Distillation(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("reserved", C.c_uint32), ("rows", C.c_uint64), ("vocabulary", C.c_uint64), ("top", C.c_uint64), ("logits", C.c_void_p),
+                ("logits_stride", C.c_int64), ("index", C.c_void_p), ("index_stride", C.c_int64), ("teacher", C.c_void_p), ("teacher_stride", C.c_int64),
+                ("labels", C.c_void_p), ("weight", C.c_void_p), ("temperature", C.c_float), ("soft", C.c_float), ("hard", C.c_float), ("reserved2", C.c_float),
+                ("losses", C.c_void_p), ("d_logits", C.c_void_p), ("d_logits_stride", C.c_int64)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("reserved", C.c_uint32), ("rows", C.c_uint64), ("vocabulary", C.c_uint64), ("logits", C.c_void_p),
+                ("logits_stride", C.c_int64), ("uniform", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p), ("tokens", C.c_void_p), ("chances", C.c_void_p)]
+
+
 class LayerIndex(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in
                 ("first_connection_index", "last_connection_index", "first_bias_connection_index",
@@ -252,6 +265,8 @@ _PROTOS = {
     "myea_b200_selective_scan": (C.c_int, [C.c_int, C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
     "myea_b200_selective_scan_backward_workspace": (C.c_size_t, [C.POINTER(Scan)]),
     "myea_b200_selective_scan_backward": (C.c_int, [C.c_int, C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_distillation_error": (C.c_int, [C.c_int, C.POINTER(Distillation), C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_sample": (C.c_int, [C.c_int, C.POINTER(Sampling), C.c_void_p, C.c_char_p, C.c_size_t]),
     "myea_b200_profile": (C.c_int, [C.c_void_p, C.c_int]),
     "myea_b200_profile_read": (C.c_int, [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_uint64),
                                          C.POINTER(C.c_double), C.c_int]),

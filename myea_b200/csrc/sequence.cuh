@@ -130,6 +130,29 @@ __device__ __forceinline__ int sequence_length(const int32_t *lengths, long long
   return lengths == nullptr ? time : min(max(lengths[b], 0), time);
 }
 
+__device__ __forceinline__ bool aligned_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// over all threads of a block of at most 512, in a fixed order; memory: 17 floats that nothing else uses meanwhile
+__device__ __forceinline__ float block_sum(float x, float *memory) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) memory[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0.f;
+  for (int k = 0; k < static_cast<int>(blockDim.x >> 5); ++k) x += memory[k];
+  return x;
+}
+__device__ __forceinline__ float block_max(float x, float *memory) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) memory[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = memory[0];
+  for (int k = 1; k < static_cast<int>(blockDim.x >> 5); ++k) x = fmaxf(x, memory[k]);
+  return x;
+}
+
 // store(column, sum over rows of part[row][column]): partial sums of blocks that ran side by side, 32 columns and 8 strands of
 // rows per block of 256 threads, the strands joined in their order
 template <typename Store>

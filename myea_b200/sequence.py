@@ -208,3 +208,52 @@ def selective_scan_backward(dy, u, delta, A, B, C_, checkpoints, D=None, z=None,
     work, size = _workspace("selective_scan_backward_workspace", s, dev)
     _call("selective_scan_backward", dev, C.byref(s), work.data_ptr() if size else None, size)
     return got
+
+
+def _rows(name, x, shape, dtype, device):
+    """address and row pitch of a [rows, columns] tensor"""
+    if x is None:
+        return None, 0
+    _check(name, x, shape, dtype, device)
+    if not _dense(x, 1):
+        raise ValueError("%s: the columns have to lie densely, strides are %s" % (name, x.stride()))
+    return x.data_ptr(), x.stride(0)
+
+
+def distillation_error(logits, index, teacher, temperature=1.0, soft=1.0, hard=0.0, labels=None, weight=None, derivatives=True, losses=None, d_logits=None):
+    """(losses [rows], d_logits [rows, vocabulary] or None): the error of `logits` against a teacher's best logits, teacher[r, k] (float32) of
+    word index[r, k] (int32, outside the vocabulary: no entry), with `soft` * temperature^2 * KL(teacher, logits) at that
+    temperature plus `hard` * cross entropy to labels (int32 [rows], outside the vocabulary: none), times weight (float32 [rows]); and its
+    derivatives, of the logits' type, unless derivatives = False.  d_logits may be `logits`."""
+    if logits.dim() != 2 or index.dim() != 2:
+        raise ValueError("logits is [rows, vocabulary], index and teacher are [rows, top]")
+    (r, v), k, dev = logits.shape, index.shape[1], logits.device
+    s = capi.Distillation(_type(logits), 0, r, v, k)
+    losses = _out(losses, (r,), torch.float32, dev)
+    d_logits = _out(d_logits, (r, v), logits.dtype, dev) if derivatives else None
+    s.logits, s.logits_stride = _rows("logits", logits, (r, v), logits.dtype, dev)
+    s.index, s.index_stride = _rows("index", index, (r, k), torch.int32, dev)
+    s.teacher, s.teacher_stride = _rows("teacher", teacher, (r, k), torch.float32, dev)
+    s.labels, s.weight = _array("labels", labels, (r,), torch.int32, dev), _array("weight", weight, (r,), torch.float32, dev)
+    s.temperature, s.soft, s.hard = temperature, soft, hard
+    s.losses = _array("losses", losses, (r,), torch.float32, dev)
+    s.d_logits, s.d_logits_stride = _rows("d_logits", d_logits, (r, v), logits.dtype, dev)
+    _call("distillation_error", dev, C.byref(s))
+    return losses, d_logits
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, chances=None):
+    """(tokens int32 [rows], chances [rows]): one token for every row of logits [rows, vocabulary], drawn with uniform (float32 [rows], in
+    [0, 1)) from what temperature, top_k (int32), top_p and min_p leave of the row, each an array of one value per row or None; and
+    the chance that it had.  temperature <= 0: the largest logit.  A row whose words are all closed (minus infinity): token -1."""
+    if logits.dim() != 2:
+        raise ValueError("logits is [rows, vocabulary]")
+    (r, v), dev = logits.shape, logits.device
+    s = capi.Sampling(_type(logits), 0, r, v)
+    tokens, chances = _out(tokens, (r,), torch.int32, dev), _out(chances, (r,), torch.float32, dev)
+    s.logits, s.logits_stride = _rows("logits", logits, (r, v), logits.dtype, dev)
+    for name, x, dtype in (("uniform", uniform, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int32), ("chances", chances, torch.float32)):
+        setattr(s, name, _array(name, x, (r,), dtype, dev))
+    _call("sample", dev, C.byref(s))
+    return tokens, chances

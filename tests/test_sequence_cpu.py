@@ -85,3 +85,36 @@ def test_tensors_off_the_gpu_are_refused():
         sequence.causal_convolution(x, w)
     with pytest.raises(ValueError, match="GPU"):
         sequence.selective_scan(x, x, torch.zeros(8, 16), torch.zeros(1, 4, 1, 16), torch.zeros(1, 4, 1, 16))
+
+
+def distillation(**kw):
+    s = capi.Distillation(capi.TYPE_F32, 0, 4, 100, 8, temperature=1.0, soft=1.0)
+    for k, n in enumerate(("logits", "index", "teacher", "losses")):
+        setattr(s, n, ADDRESS + 1024 * k)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+def sampling(**kw):
+    s = capi.Sampling(capi.TYPE_F32, 0, 4, 100)
+    for k, n in enumerate(("logits", "uniform", "tokens")):
+        setattr(s, n, ADDRESS + 1024 * k)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+@pytest.mark.parametrize("change,word", [(dict(type=9), "type"), (dict(rows=1 << 31), "dimension"), (dict(vocabulary=1 << 31), "dimension"), (dict(top=0), "entries"),
+                                         (dict(top=1025), "entries"), (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+                                         (dict(temperature=float("inf")), "temperature"), (dict(vocabulary=0), "vocabulary"), (dict(logits=None), "logits"),
+                                         (dict(index=None), "index"), (dict(teacher=None), "teacher"), (dict(losses=None), "losses")])
+def test_distillation_refusals(change, word):
+    assert word in refused("distillation_error", distillation(**change))
+
+
+@pytest.mark.parametrize("change,word", [(dict(type=9), "type"), (dict(rows=1 << 31), "dimension"), (dict(vocabulary=1 << 31), "dimension"), (dict(vocabulary=0), "vocabulary"),
+                                         (dict(logits=None), "logits"), (dict(uniform=None), "uniform"), (dict(tokens=None), "tokens")])
+def test_sampling_refusals(change, word):
+    assert word in refused("sample", sampling(**change))
+    assert refused("sample", None) and refused("distillation_error", None)
