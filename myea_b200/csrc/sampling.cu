@@ -1,242 +1,459 @@
 // Draws one token per row from what temperature, top-k, top-p and min-p leave of it (defined at myea_sampling in myea_b200.h).
 //
 // All three limits keep a prefix of the row ordered by falling logit and rising index, so what is kept is a threshold on the
-// logit and, among those equal to it, on the index.  The threshold is found without sorting: radix selection on the logits'
-// bits (mapped to integers of the same order), 11, 11 and 10 at a time, with a histogram of counts and weights per digit.
-// Weights are 64-bit integers, w * 2^shift: their sums are exact whatever the order of the atomics, and the same draw is
-// made every time.
+// logit and, among those equal to it, on the index.  The threshold is found without sorting, by histograms of counts or
+// weights: first 2048 bins in the distance from the maximum, which spread the words of any ordinary row, then bins in the logits' bits
+// (mapped to integers of the same order) within the bin that holds the threshold, until one value is left.
+//
+// Weights are integers, w * 2^shift: their sums are exact whatever the order of the atomics, and the same draw is made every
+// time.  A draw from 1e5 words goes through as many borders, so a weight good to 24 bits would move a token of every few
+// hundred rows; these are good to 2^-44 or better.  2^t is a table of 2^(k / 256) times the polynomial 1 + r + ... of the rest
+// |r| < 2^-9.5 (its first term left out is below 2^-54), in 64-bit floating point, which this chip does at half the 32-bit rate.
+//
+// A cluster of up to eight blocks takes a row, each keeps its slice in shared memory, so the row is read from memory once whatever
+// is asked of it; rows beyond the clusters' memory are read again in every pass.  A warp works on a contiguous part of a slice, so
+// that the draw, which goes by rising index, finds its word from the warps' sums and one warp's walk over its part.
+#include <cooperative_groups.h>
+
 #include "sequence.cuh"
 
 namespace myea {
 namespace {
 
+namespace cg = cooperative_groups;
 using u64 = unsigned long long;
-constexpr int kThreads = 1024;
-constexpr int kBins = 2048;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kParts = 8;
+constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
+
+template <typename T> struct Pack { static constexpr int N = 16 / sizeof(T); uint4 v; };
 
 // integers in the order of the floats; 0: a closed word
 __device__ __forceinline__ uint32_t key_of(float x) {
   if (!(x > -INFINITY)) return 0;
-  if (x == 0.f) x = 0.f;   // both zeros are equal
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);   // (both zeros are equal)
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
-
-struct Row {
-  float m, inv;        // largest logit
-  double per;          // 1 / temperature
-  int shift;
-  // the weight of a logit as an integer
-  __device__ __forceinline__ u64 weight(float x) const {
-    if (!(x > -INFINITY)) return 0;
-    const double w = x == m ? 1.0 : m == INFINITY ? 0.0 : exp((static_cast<double>(x) - static_cast<double>(m)) * per);
-    return static_cast<u64>(__double2ll_rn(ldexp(w, shift)));
-  }
-};
-
-__device__ __forceinline__ u64 warp_sum(u64 x) {
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
-  return x;
-}
-
-struct Shared {
-  unsigned int count[kBins];
-  u64 mass[kBins];
-  u64 warp[32];
-  float warp_m[32];
-  int warp_i[32];
-  int digit;
-  u64 before_count, before_mass, bin_count, bin_mass;
-  int token;
-  u64 chance;
-};
 
 // What is kept: keys above `key`, and those equal to it up to index `last`
 struct Kept {
   uint32_t key = 1;
-  long long last = 1ll << 62;
-  __device__ __forceinline__ bool has(uint32_t k, long long i) const { return k > key || (k == key && i <= last); }
+  int last = 0x7fffffff;
+  __device__ __forceinline__ bool has(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
 };
 
-// The first index, in rising order, at which the running sum of f(index) exceeds `target`; -1: none does.  before, own: the sum in front of it and its own
-template <typename F> __device__ long long first_beyond(Shared &s, long long from, long long to, u64 target, F f, u64 *own) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  while (true) {
-    const long long n = to - from, share = (n + 31) / 32, lo = from + share * warp, hi = min(lo + share, to);
-    u64 sum = 0;
-    for (long long i = lo + lane; i < hi; i += 32) sum += f(i);
-    sum = warp_sum(sum);
-    __syncthreads();
-    if (lane == 0) s.warp[warp] = sum;
-    __syncthreads();
-    int w = 0;
-    u64 before = 0;
-    for (; w < 32; ++w) {
-      if (before + s.warp[w] > target) break;
-      before += s.warp[w];
-    }
-    if (w == 32) return -1;
-    if (share == 1) {
-      if (own != nullptr) *own = s.warp[w];
-      __syncthreads();
-      return from + w;
-    }
-    target -= before;
-    from += share * w;
-    to = min(from + share, to);
-    __syncthreads();
-  }
-}
+struct alignas(16) Shared {
+  unsigned int count[kBins], low[kBins], high[kBins];   // of a histogram: words, and their weights' lower and upper 32 bits
+  double table[256];                                    // 2^(k / 256)
+  u64 warp[kWarps];
+  float warp_m[kWarps];
+  float m;
+  unsigned int key_min, key_max;
+  int best, found;
+  u64 own;
+  // the bin that holds a limit
+  int bin;
+  u64 before_count, before_mass, bin_count, bin_mass, total_mass;
+  u64 scan_count[kWarps], scan_mass[kWarps];
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling a, int shift) {
-  __shared__ Shared s;
-  const long long row = blockIdx.x, V = static_cast<long long>(a.vocabulary);
-  const T *x = static_cast<const T *>(a.logits) + row * a.logits_stride;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float temperature = a.temperature == nullptr ? 1.f : a.temperature[row];
-  const float top_p = a.top_p == nullptr ? 1.f : a.top_p[row], min_p = a.min_p == nullptr ? 0.f : a.min_p[row];
-  const long long top_k = a.top_k == nullptr ? 0 : a.top_k[row];
-  const bool greedy = !(temperature > 0.f);
+template <typename T, bool RES> struct Draw {
+  static constexpr int E = Pack<T>::N;
+  cg::cluster_group cluster;
+  Shared &s;
+  const T *x;          // the row
+  uint4 *slice;        // this block's vectors of it (RES)
+  int V, lead;         // words; elements by which the first vector begins before the row
+  int first, last;     // this block's vectors
+  int from, to;        // this warp's
+  int parts, part, lane, warp;
+  float m, half_scale; // the maximum; (m - x) / temperature = (m / 2 - x / 2) * half_scale
+  double md, per;      // 256 log2(e) / temperature
+  int shift;
+  float beyond;        // distances from here on weigh nothing
+  u64 warps[4], upto_warps;   // of total(): up to four warps' sums, and the running sum up to them
 
-  float m = -INFINITY;
-  long long at = -1;
-  for (long long i = tid; i < V; i += kThreads) {
-    const float e = to_float(x[i]);
-    if (e > m) { m = e; at = i; }
-  }
+  __device__ __forceinline__ Draw(Shared &s_) : cluster(cg::this_cluster()), s(s_) {}
+
+  // vector v of the row, -infinity where there is no word
+  __device__ __forceinline__ Pack<T> from_memory(int v) const {
+    const long long at = static_cast<long long>(v) * E - lead;
+    Pack<T> p;
+    if (at >= 0 && at + E <= V) {
+      p.v = *reinterpret_cast<const uint4 *>(x + at);
+    } else {
+      T *e = reinterpret_cast<T *>(&p.v);
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) {
-    const float o = __shfl_xor_sync(0xffffffffu, m, k);
-    const long long oi = __shfl_xor_sync(0xffffffffu, at, k);
-    if (o > m || (o == m && oi < at && oi >= 0)) { m = o; at = oi; }
-  }
-  if (lane == 0) { s.warp_m[warp] = m; s.warp_i[warp] = static_cast<int>(at); }
-  __syncthreads();
-  m = s.warp_m[0];
-  at = s.warp_i[0];
-  for (int k = 1; k < 32; ++k)
-    if (s.warp_m[k] > m || (s.warp_m[k] == m && s.warp_i[k] < at && s.warp_i[k] >= 0)) { m = s.warp_m[k]; at = s.warp_i[k]; }
-  if (at < 0 || greedy) {
-    if (tid == 0) {
-      a.tokens[row] = static_cast<int>(at);
-      if (a.chances != nullptr) a.chances[row] = at < 0 ? 0.f : 1.f;
+      for (int k = 0; k < E; ++k) e[k] = at + k >= 0 && at + k < V ? x[at + k] : from_float<T>(-INFINITY);
     }
-    return;
+    return p;
   }
-  Row r;
-  r.m = m; r.per = 1.0 / static_cast<double>(temperature); r.shift = shift;
+  __device__ __forceinline__ void words(int v, float (&e)[E]) const {
+    Pack<T> p;
+    if constexpr (RES) p.v = slice[v - first];
+    else p = from_memory(v);
+    const T *w = reinterpret_cast<const T *>(&p.v);
+#pragma unroll
+    for (int k = 0; k < E; ++k) e[k] = to_float(w[k]);
+  }
+  __device__ __forceinline__ float distance(float e) const { return (0.5f * m - 0.5f * e) * half_scale; }
+  // the weight of a word as an integer
+  __device__ __forceinline__ u64 weight(float e) const {
+    if (e == m) return 1ull << shift;
+    if (!(distance(e) < beyond) || m == INFINITY) return 0;
+    constexpr double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's lower bits are the nearest integer
+    constexpr double c1 = kLn2 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6, c4 = c1 * c1 * c1 * c1 / 24;
+    const double d = static_cast<double>(e) - md;
+    const double z = fma(d, per, magic);
+    const int i = __double2loint(z);
+    const double r = fma(d, per, magic - z);
+    double q = fma(fma(fma(fma(r, c4, c3), r, c2), r, c1), r, 1.0);
+    q *= s.table[i & 255];
+    const u64 bits = static_cast<u64>(__double_as_longlong(q));
+    const int right = 52 - (static_cast<int>(bits >> 52) - 1023) - (i >> 8) - shift;   // (q > 0; i <= 0)
+    return right > 63 ? 0 : ((bits & ((1ull << 52) - 1)) | (1ull << 52)) >> right;
+  }
+  // f(word, its index) for this warp's words, lanes side by side
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll 2
+    for (int v = from + lane; v < to; v += 32) {
+      float e[E];
+      words(v, e);
+#pragma unroll
+      for (int k = 0; k < E; ++k) f(e[k], v * E + k - lead);
+    }
+  }
+  static __device__ __forceinline__ u64 warp_sum(u64 y) {
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
+    return y;
+  }
+  // Sums of f over the row's words by warps (put into s.warp): their total, in every block
+  template <typename F> __device__ u64 total(F f) {
+    u64 sum = 0;
+    each([&](float e, int i) { sum += f(e, i); });
+    sum = warp_sum(sum);
+    if (lane == 0) s.warp[warp] = sum;
+    cluster.sync();
+    // up to four neighbouring warps' sums per lane, and the running sum up to them
+    const int each_lane = (parts * kWarps + 31) / 32;
+    upto_warps = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = lane * each_lane + j;
+      warps[j] = j < each_lane && k < parts * kWarps ? cluster.map_shared_rank(&s, k / kWarps)->warp[k % kWarps] : 0;
+      upto_warps += warps[j];
+    }
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const u64 o = __shfl_up_sync(0xffffffffu, upto_warps, k);
+      if (lane >= k) upto_warps += o;
+    }
+    return __shfl_sync(0xffffffffu, upto_warps, 31);
+  }
+  // The first index, in rising order, at which the running sum of f exceeds `target` (below the total, after total(f)), and f there:
+  // known to every block behind the next cluster.sync(), in s.found and s.own
+  template <typename F> __device__ void find(u64 target, F f) {
+    const int each_lane = (parts * kWarps + 31) / 32;
+    const int with = __ffs(__ballot_sync(0xffffffffu, upto_warps > target)) - 1;   // the lane that has the warp
+    u64 before = upto_warps - (warps[0] + warps[1] + warps[2] + warps[3]);
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (at == j && before + warps[j] <= target) {
+        before += warps[j];
+        ++at;
+      }
+    before = __shfl_sync(0xffffffffu, before, with);
+    at = with * each_lane + __shfl_sync(0xffffffffu, at, with);
+    if (at != part * kWarps + warp) return;
+    for (int v0 = from; v0 < to; v0 += 32) {
+      const int v = v0 + lane;
+      float e[E];
+      u64 own[E], sum = 0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) own[k] = 0;
+      if (v < to) {
+        words(v, e);
+#pragma unroll
+        for (int k = 0; k < E; ++k) { own[k] = f(e[k], v * E + k - lead); sum += own[k]; }
+      }
+      u64 upto = sum;
+#pragma unroll
+      for (int k = 1; k < 32; k <<= 1) {
+        const u64 o = __shfl_up_sync(0xffffffffu, upto, k);
+        if (lane >= k) upto += o;
+      }
+      const unsigned beyond_ = __ballot_sync(0xffffffffu, before + upto > target);
+      if (beyond_ != 0) {
+        if (lane == __ffs(beyond_) - 1) {
+          u64 run = before + upto - sum;
+          int k = 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (k == j) {
+              if (run + own[j] > target) break;
+              run += own[j];
+              ++k;
+            }
+          u64 mine = 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (k == j) mine = own[j];
+          for (int o = 0; o < parts; ++o) {
+            Shared *to_ = cluster.map_shared_rank(&s, o);
+            to_->found = v * E + k - lead;
+            to_->own = mine;
+          }
+        }
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
 
-  Kept kept;
-  // keeps the first n words (by count), or those before which less than `mass` lies
-  const auto limit = [&](bool by_mass, u64 target) {
-    uint32_t prefix = 0;
-    u64 before_count = 0, before_mass = 0;
-    int low = 21;
-    for (int round = 0; round < 3; ++round) {
-      const int bits = round < 2 ? 11 : 10;
-      low = round == 0 ? 21 : round == 1 ? 10 : 0;
-      __syncthreads();
-      for (int k = tid; k < kBins; k += kThreads) { s.count[k] = 0; s.mass[k] = 0; }
-      __syncthreads();
-      for (long long i = tid; i < V; i += kThreads) {
-        const float e = to_float(x[i]);
-        const uint32_t key = key_of(e);
-        if (key == 0 || !kept.has(key, i) || (round > 0 && (key >> (low + bits)) != prefix)) continue;
-        const uint32_t digit = (key >> low) & ((1u << bits) - 1);
-        atomicAdd(&s.count[digit], 1u);
-        if (by_mass) atomicAdd(&s.mass[digit], r.weight(e));
+  // Histogram of the words for which bin(word, index) >= 0, over the cluster, and the bin that holds the limit: the first, from bin 0
+  // on, with `target` words (or `target` of weight) up to its end.  part_of_all < 1: the target is that part of the whole weight.
+  // s.bin is -1 where there is less.  On entry before_count / before_mass: what lies in front of bin 0.
+  template <typename F> __device__ void limit_bin(bool by_mass, double part_of_all, u64 target, u64 before_count, u64 before_mass, F bin) {
+    for (int k = threadIdx.x; k < kBins; k += kThreads) s.count[k] = s.low[k] = s.high[k] = 0;
+    if (threadIdx.x == 0) { s.bin = -1; s.total_mass = 0; }
+    __syncthreads();
+    each([&](float e, int i) {
+      const int b = bin(e, i);
+      if (b < 0) return;
+      atomicAdd(&s.count[b], 1u);
+      if (by_mass) {
+        const u64 w = weight(e);
+        const unsigned l = static_cast<unsigned>(w);
+        const unsigned old = atomicAdd(&s.low[b], l);
+        const unsigned up = static_cast<unsigned>(w >> 32) + (old + l < l ? 1u : 0u);
+        if (up != 0) atomicAdd(&s.high[b], up);
       }
-      __syncthreads();
-      if (tid == 0) {
-        int d = (1 << bits) - 1;
-        for (; d >= 0; --d) {
-          if (s.count[d] == 0) continue;
-          if (by_mass ? before_mass + s.mass[d] >= target : before_count + s.count[d] >= target) break;
-          before_count += s.count[d];
-          before_mass += s.mass[d];
-        }
-        s.digit = d;
-        if (d >= 0) {
-          s.before_count = before_count; s.before_mass = before_mass;
-          s.bin_count = s.count[d]; s.bin_mass = s.mass[d];
-        }
+    });
+    cluster.sync();
+    constexpr int B = kBins / kThreads;
+    u64 c[B], w[B], sum_c = 0, sum_w = 0;
+#pragma unroll
+    for (int k = 0; k < B; ++k) { c[k] = 0; w[k] = 0; }
+    for (int o = 0; o < parts; ++o) {
+      const Shared *h = cluster.map_shared_rank(&s, o);
+      const uint4 n = *reinterpret_cast<const uint4 *>(&h->count[threadIdx.x * B]);
+      c[0] += n.x; c[1] += n.y; c[2] += n.z; c[3] += n.w;
+      if (by_mass) {
+        const uint4 l = *reinterpret_cast<const uint4 *>(&h->low[threadIdx.x * B]), u = *reinterpret_cast<const uint4 *>(&h->high[threadIdx.x * B]);
+        w[0] += l.x + (static_cast<u64>(u.x) << 32); w[1] += l.y + (static_cast<u64>(u.y) << 32);
+        w[2] += l.z + (static_cast<u64>(u.z) << 32); w[3] += l.w + (static_cast<u64>(u.w) << 32);
       }
-      __syncthreads();
-      if (s.digit < 0) return;   // fewer words than the limit
-      prefix = (prefix << bits) | static_cast<uint32_t>(s.digit);
-      before_count = s.before_count;
-      before_mass = s.before_mass;
     }
+#pragma unroll
+    for (int k = 0; k < B; ++k) { sum_c += c[k]; sum_w += w[k]; }
+    u64 upto_c = sum_c, upto_w = sum_w;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const u64 oc = __shfl_up_sync(0xffffffffu, upto_c, k), ow = __shfl_up_sync(0xffffffffu, upto_w, k);
+      if (lane >= k) { upto_c += oc; upto_w += ow; }
+    }
+    if (lane == 31) { s.scan_count[warp] = upto_c; s.scan_mass[warp] = upto_w; }
+    __syncthreads();
+    u64 all_w = 0;
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warp) { before_count += s.scan_count[k]; before_mass += s.scan_mass[k]; }
+      all_w += s.scan_mass[k];
+    }
+    if (part_of_all < 1.0) target = static_cast<u64>(ceil(part_of_all * static_cast<double>(all_w)));
+    before_count += upto_c - sum_c;
+    before_mass += upto_w - sum_w;
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      if (c[k] != 0) {
+        // the first bin of words with enough up to its end
+        const bool enough = by_mass ? before_mass + w[k] >= target : before_count + c[k] >= target;
+        const bool was = by_mass ? before_count != 0 && before_mass >= target : before_count >= target;
+        if (enough && !was) {
+          s.bin = threadIdx.x * B + k;
+          s.before_count = before_count;
+          s.before_mass = before_mass;
+          s.bin_count = c[k];
+          s.bin_mass = w[k];
+        }
+      }
+      before_count += c[k];
+      before_mass += w[k];
+    }
+    if (threadIdx.x == 0) s.total_mass = target;
+    cluster.sync();   // nobody clears its bins while others read them
+  }
+
+  // keeps the first `target` words, or those before which less than the part `part_of_all` of the weight of what was kept lies
+  __device__ void limit(Kept &kept, bool by_mass, double part_of_all, u64 target) {
+    // bins by distance: 64 to a unit, of the logits for counts and of the logarithm of the weights for weights
+    const float scale = by_mass ? 64.f * half_scale : 128.f;
+    const auto far = [&](float e) {
+      const float t = (0.5f * m - 0.5f * e) * scale;
+      return e == m ? 0 : t < static_cast<float>(kBins - 1) ? static_cast<int>(t) : kBins - 1;
+    };
+    const Kept was = kept;
+    limit_bin(by_mass, by_mass ? part_of_all : 1.0, target, 0, 0, [&](float e, int i) { const uint32_t k = key_of(e); return k != 0 && was.has(k, i) ? far(e) : -1; });
+    if (s.bin < 0) return;   // fewer words than that
+    target = s.total_mass;
+    const int bin = s.bin;
+    // the logits in that bin
+    if (threadIdx.x == 0) { s.key_min = 0xffffffffu; s.key_max = 0; }
+    __syncthreads();
+    uint32_t lowest = 0xffffffffu, highest = 0;
+    each([&](float e, int i) {
+      const uint32_t k = key_of(e);
+      if (k != 0 && was.has(k, i) && far(e) == bin) { lowest = min(lowest, k); highest = max(highest, k); }
+    });
+    lowest = __reduce_min_sync(0xffffffffu, lowest);
+    highest = __reduce_max_sync(0xffffffffu, highest);
+    if (lane == 0) { atomicMin(&s.key_min, lowest); atomicMax(&s.key_max, highest); }
+    cluster.sync();
+    for (int o = 0; o < parts; ++o) {
+      const Shared *h = cluster.map_shared_rank(&s, o);
+      lowest = min(lowest, h->key_min);
+      highest = max(highest, h->key_max);
+    }
+    while (lowest != highest) {
+      int narrow = 0;
+      while (((highest - lowest) >> narrow) >= kBins) ++narrow;
+      const uint32_t lo = lowest, hi = highest;
+      const u64 before_count = s.before_count, before_mass = s.before_mass;
+      __syncthreads();
+      limit_bin(by_mass, 1.0, target, before_count, before_mass,
+                [&](float e, int i) { const uint32_t k = key_of(e); return k >= lo && k <= hi && was.has(k, i) ? static_cast<int>((hi - k) >> narrow) : -1; });
+      highest = hi - (static_cast<uint32_t>(s.bin) << narrow);
+      lowest = highest - ((1u << narrow) - 1);
+      lowest = lowest < lo || lowest > highest ? lo : lowest;
+      if (narrow == 0) lowest = highest;
+    }
+    const uint32_t key = highest;
     // of the words equal to the threshold
     u64 ties;
     if (by_mass) {
-      const u64 each = s.bin_count > 0 ? s.bin_mass / s.bin_count : 0;
-      ties = each == 0 ? s.bin_count : (target > before_mass ? (target - before_mass + each - 1) / each : 0);
-      if (before_count == 0 && ties == 0) ties = 1;
+      const u64 one = s.bin_mass / s.bin_count;
+      ties = one == 0 ? s.bin_count : target > s.before_mass ? (target - s.before_mass + one - 1) / one : 0;
+      if (s.before_count == 0 && ties == 0) ties = 1;
     } else {
-      ties = target - before_count;
+      ties = target - s.before_count;
     }
     if (ties < s.bin_count) {
-      const Kept was = kept;
-      const uint32_t key = prefix;
-      const long long last = first_beyond(s, 0, V, ties - 1, [&](long long i) -> u64 { const uint32_t k = key_of(to_float(x[i])); return k == key && was.has(k, i); }, nullptr);
-      kept.last = last;
+      const auto tie = [&](float e, int i) -> u64 { const uint32_t k = key_of(e); return k == key && was.has(k, i) ? 1 : 0; };
+      if (ties > 0) {
+        total(tie);
+        find(ties - 1, tie);
+        cluster.sync();
+        kept.last = s.found;
+        kept.key = key;
+      } else {
+        kept.key = key;
+        kept.last = -1;
+      }
+    } else if (key > kept.key) {
       kept.key = key;
-    } else if (prefix > kept.key) {
-      kept.key = prefix;
-      kept.last = 1ll << 62;
+      kept.last = 0x7fffffff;
     }
-    __syncthreads();
-  };
-  const auto sum_kept = [&]() {
-    u64 sum = 0;
-    for (long long i = tid; i < V; i += kThreads) {
-      const float e = to_float(x[i]);
-      const uint32_t k = key_of(e);
-      if (k != 0 && kept.has(k, i)) sum += r.weight(e);
-    }
-    sum = warp_sum(sum);
-    __syncthreads();
-    if (lane == 0) s.warp[warp] = sum;
-    __syncthreads();
-    sum = 0;
-    for (int k = 0; k < 32; ++k) sum += s.warp[k];
-    return sum;
-  };
-  if (top_k > 0 && top_k < V) limit(false, static_cast<u64>(top_k));
-  u64 total = sum_kept();
-  if (top_p < 1.f) {
-    const double part = top_p > 0.f ? static_cast<double>(top_p) * static_cast<double>(total) : 0.0;
-    limit(true, static_cast<u64>(ceil(part)));
+    __syncthreads();   // what has been read here is written by the next limit
   }
-  // the least weight, as an integer of the same scale
-  u64 least = 0;
-  if (min_p > 0.f) least = min_p >= 1.f ? 1ull << shift : static_cast<u64>(ceil(ldexp(static_cast<double>(min_p), shift)));
-  const auto weigh = [&](long long i) -> u64 {
-    const float e = to_float(x[i]);
+};
+
+template <typename T, bool RES>
+__global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling a, int shift) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  Shared &s = *reinterpret_cast<Shared *>(dynamic);
+  Draw<T, RES> d(s);
+  constexpr int E = Pack<T>::N;
+  d.parts = static_cast<int>(d.cluster.num_blocks());
+  d.part = static_cast<int>(d.cluster.block_rank());
+  d.lane = threadIdx.x & 31;
+  d.warp = threadIdx.x >> 5;
+  const long long row = blockIdx.x / d.parts;
+  d.x = static_cast<const T *>(a.logits) + row * a.logits_stride;
+  d.V = static_cast<int>(a.vocabulary);
+  d.lead = static_cast<int>(reinterpret_cast<uintptr_t>(d.x) % 16 / sizeof(T));
+  const long long vectors = (d.lead + static_cast<long long>(d.V) + E - 1) / E;
+  d.first = static_cast<int>(vectors * d.part / d.parts);
+  d.last = static_cast<int>(vectors * (d.part + 1) / d.parts);
+  d.slice = reinterpret_cast<uint4 *>(dynamic + sizeof(Shared));
+  const int share = (d.last - d.first + kWarps - 1) / kWarps;
+  d.from = min(d.first + d.warp * share, d.last);
+  d.to = min(d.from + share, d.last);
+  const float temperature = a.temperature == nullptr ? 1.f : a.temperature[row];
+  const float top_p = a.top_p == nullptr ? 1.f : a.top_p[row], min_p = a.min_p == nullptr ? 0.f : a.min_p[row], uniform = a.uniform[row];
+  const int top_k = a.top_k == nullptr ? 0 : a.top_k[row];
+
+  float m = -INFINITY;
+  constexpr int U = 4;
+  for (int v = d.from + d.lane; v < d.to; v += 32 * U) {
+    Pack<T> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + 32 * u < d.to) p[u] = d.from_memory(v + 32 * u);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + 32 * u < d.to) {
+        if constexpr (RES) d.slice[v + 32 * u - d.first] = p[u].v;
+        const T *e = reinterpret_cast<const T *>(&p[u].v);
+#pragma unroll
+        for (int k = 0; k < E; ++k) m = fmaxf(m, to_float(e[k]));   // (NaN is passed over)
+      }
+  }
+  if (threadIdx.x < 256) s.table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 256.0);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+  if (d.lane == 0) s.warp_m[d.warp] = m;
+  if (threadIdx.x == 0) s.best = 0x7fffffff;
+  __syncthreads();
+  for (int k = 0; k < kWarps; ++k) m = fmaxf(m, s.warp_m[k]);
+  if (threadIdx.x == 0) s.m = m;
+  d.cluster.sync();
+  for (int k = 0; k < d.parts; ++k) m = fmaxf(m, d.cluster.map_shared_rank(&s, k)->m);
+  if (m == -INFINITY || !(temperature > 0.f)) {
+    int best = 0x7fffffff;
+    if (m != -INFINITY) d.each([&](float e, int i) { if (e == m) best = min(best, i); });
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (d.lane == 0) atomicMin(&s.best, best);
+    d.cluster.sync();
+    if (d.part == 0 && threadIdx.x == 0) {
+      for (int k = 0; k < d.parts; ++k) best = min(best, d.cluster.map_shared_rank(&s, k)->best);
+      a.tokens[row] = m == -INFINITY ? -1 : best;
+      if (a.chances != nullptr) a.chances[row] = m == -INFINITY ? 0.f : 1.f;
+    }
+    d.cluster.sync();
+    return;
+  }
+  d.m = m;
+  d.md = static_cast<double>(m);
+  d.half_scale = 2.f / temperature;
+  d.per = 256.0 * kLog2e / static_cast<double>(temperature);
+  d.shift = shift;
+  d.beyond = static_cast<float>((shift + 1) * kLn2) + 0.5f;
+
+  Kept kept;
+  if (top_k > 0 && top_k < d.V) d.limit(kept, false, 1.0, static_cast<u64>(top_k));
+  if (top_p < 1.f) d.limit(kept, true, top_p > 0.f ? static_cast<double>(top_p) : 0.0, 0);
+  // the least weight, as an integer of the same scale, and the distance behind which no weight reaches it
+  u64 least = 1;
+  float reach = d.beyond;
+  if (min_p > 0.f) {
+    least = min_p >= 1.f ? 1ull << shift : static_cast<u64>(ceil(ldexp(static_cast<double>(min_p), shift)));
+    reach = fminf(reach, -logf(min_p) * 1.0001f + 1e-3f);
+  }
+  const auto weigh = [&](float e, int i) -> u64 {
+    if (!(d.distance(e) < reach) && e != m) return 0;
     const uint32_t k = key_of(e);
     if (k == 0 || !kept.has(k, i)) return 0;
-    const u64 w = r.weight(e);
+    const u64 w = d.weight(e);
     return w >= least ? w : 0;
   };
-  u64 sum = 0;
-  for (long long i = tid; i < V; i += kThreads) sum += weigh(i);
-  sum = warp_sum(sum);
-  __syncthreads();
-  if (lane == 0) s.warp[warp] = sum;
-  __syncthreads();
-  total = 0;
-  for (int k = 0; k < 32; ++k) total += s.warp[k];
-  const float uniform = a.uniform[row];
+  const u64 total = d.total(weigh);
   u64 target = uniform > 0.f ? static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(total)) : 0;
   if (target >= total) target = total - 1;
-  u64 own = 0;
-  const long long token = first_beyond(s, 0, V, target, weigh, &own);
-  if (tid == 0) {
-    a.tokens[row] = static_cast<int>(token);
-    if (a.chances != nullptr) a.chances[row] = static_cast<float>(static_cast<double>(own) / static_cast<double>(total));
+  d.find(target, weigh);
+  d.cluster.sync();
+  if (d.part == 0 && threadIdx.x == 0) {
+    a.tokens[row] = s.found;
+    if (a.chances != nullptr) a.chances[row] = static_cast<float>(static_cast<double>(s.own) / static_cast<double>(total));
   }
 }
 
@@ -247,6 +464,7 @@ const char *check(const myea_sampling *s) {
   if (s->rows == 0) return nullptr;
   if (s->vocabulary == 0) return "sample: an empty vocabulary";
   if (s->logits == nullptr || s->uniform == nullptr || s->tokens == nullptr) return "sample: logits, uniform or tokens is missing";
+  if (s->rows * kParts > 0x7fffffffull) return "sample: more rows than one launch takes";
   return nullptr;
 }
 
@@ -255,6 +473,33 @@ int shift_for(uint64_t vocabulary) {
   int bits = 0;
   while ((uint64_t(1) << bits) < vocabulary) ++bits;
   return 62 - bits < 51 ? 62 - bits : 51;
+}
+
+template <typename T, bool RES> cudaError_t launch(const myea_sampling &a, int parts, size_t smem, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(sampling_kernel<T, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows * parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sampling_kernel<T, RES>, a, shift_for(a.vocabulary));
+}
+
+template <typename T> cudaError_t launch(const myea_sampling &a, cudaStream_t stream) {
+  // a slice of at most 64 KB leaves room for two blocks on an SM; more blocks per row while the rows leave SMs idle and a
+  // slice has 4096 words
+  const uint64_t bytes = a.vocabulary * sizeof(T) + 32;
+  int parts = 1;
+  while (parts < kParts && (bytes / parts > (64u << 10) || (a.rows * parts * 2 <= 2 * kSms && a.vocabulary / (parts * 2) >= 4096))) parts *= 2;
+  const size_t slice = (bytes / parts + 64) / 16 * 16;
+  if (sizeof(Shared) + slice > (200u << 10)) return launch<T, false>(a, parts, sizeof(Shared), stream);
+  return launch<T, true>(a, parts, sizeof(Shared) + slice, stream);
 }
 
 }  // namespace
@@ -266,8 +511,9 @@ extern "C" int myea_b200_sample(int device, const myea_sampling *s, void *stream
   if (s->rows == 0) return MYEA_OK;
   DeviceScope scope(device);
   if (!scope.ok) return refuse(error_message, error_capacity, MYEA_E_CUDA, "sample: no such device");
-  with_type(s->type, [&](auto t) {
-    sampling_kernel<decltype(t)><<<static_cast<unsigned>(s->rows), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(*s, shift_for(s->vocabulary));
-  });
+  cudaError_t e = cudaSuccess;
+  with_type(s->type, [&](auto t) { e = launch<decltype(t)>(*s, static_cast<cudaStream_t>(stream)); });
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  if (e != cudaSuccess) return refuse(error_message, error_capacity, MYEA_E_CUDA, "sample: the launch was refused");
   return launched(error_message, error_capacity, "sample");
 }
