@@ -257,16 +257,16 @@ _PROTOS = {
                                     C.c_void_p, C.c_int, C.POINTER(C.c_float), C.c_int]),
     "myea_b200_gemm_nt_static": (C.c_int, [C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p,
                                            C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]),
-    "myea_b200_causal_convolution": (C.c_int, [C.c_int, C.POINTER(Convolution), C.c_void_p, C.c_char_p, C.c_size_t]),
-    "myea_b200_causal_convolution_backward_workspace": (C.c_size_t, [C.POINTER(Convolution)]),
-    "myea_b200_causal_convolution_backward": (C.c_int, [C.c_int, C.POINTER(Convolution), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
-    "myea_b200_selective_scan_checkpoint_bytes": (C.c_size_t, [C.POINTER(Scan)]),
-    "myea_b200_selective_scan_workspace": (C.c_size_t, [C.POINTER(Scan)]),
-    "myea_b200_selective_scan": (C.c_int, [C.c_int, C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
-    "myea_b200_selective_scan_backward_workspace": (C.c_size_t, [C.POINTER(Scan)]),
-    "myea_b200_selective_scan_backward": (C.c_int, [C.c_int, C.POINTER(Scan), C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
-    "myea_b200_distillation_error": (C.c_int, [C.c_int, C.POINTER(Distillation), C.c_void_p, C.c_char_p, C.c_size_t]),
-    "myea_b200_sample": (C.c_int, [C.c_int, C.POINTER(Sampling), C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_causal_convolution": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_causal_convolution_backward_workspace": (C.c_size_t, [C.c_void_p]),
+    "myea_b200_causal_convolution_backward": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_selective_scan_checkpoint_bytes": (C.c_size_t, [C.c_void_p]),
+    "myea_b200_selective_scan_workspace": (C.c_size_t, [C.c_void_p]),
+    "myea_b200_selective_scan": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_selective_scan_backward_workspace": (C.c_size_t, [C.c_void_p]),
+    "myea_b200_selective_scan_backward": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_distillation_error": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "myea_b200_sample": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
     "myea_b200_profile": (C.c_int, [C.c_void_p, C.c_int]),
     "myea_b200_profile_read": (C.c_int, [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_uint64),
                                          C.POINTER(C.c_double), C.c_int]),

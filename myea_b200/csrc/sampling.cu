@@ -2,7 +2,7 @@
 //
 // All three limits keep a prefix of the row ordered by falling logit and rising index, so what is kept is a threshold on the
 // logit and, among those equal to it, on the index.  The threshold is found without sorting, by histograms of counts or
-// weights: first 2048 bins in the distance from the maximum, which spread the words of any ordinary row, then bins in the logits' bits
+// weights: first 1024 bins in the distance from the maximum, which spread the words of any ordinary row, then bins in the logits' bits
 // (mapped to integers of the same order) within the bin that holds the threshold, until one value is left.
 //
 // Weights are integers, w * 2^shift: their sums are exact whatever the order of the atomics, and the same draw is made every
@@ -22,27 +22,43 @@ namespace {
 
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kParts = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kParts = 8, kList = 1024;
+static_assert(kThreads == 256, "a thread makes one entry of the table");
 constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
 template <typename T> struct Pack { static constexpr int N = 16 / sizeof(T); uint4 v; };
 
-// integers in the order of the floats; 0: a closed word
+// integers in the order of the floats
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (!(x > -INFINITY)) return 0;
   const uint32_t b = __float_as_uint(x + 0.f);   // (both zeros are equal)
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// What is kept: keys above `key`, and those equal to it up to index `last`
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key); }
+
+// What is kept: words above `value`, and those equal to it up to index `last` (closed words, -infinity and NaN, never)
 struct Kept {
-  uint32_t key = 1;
-  int last = 0x7fffffff;
-  __device__ __forceinline__ bool has(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
+  float value = -INFINITY;
+  int last = -1;
+  __device__ __forceinline__ bool has(float e, int i) const { return e > value || (e == value && i <= last); }
 };
 
+// the largest of a vector's words, NaN passed over
+__device__ __forceinline__ float largest(const uint4 &v, float) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+template <typename H2, typename H> __device__ __forceinline__ float largest_half(const uint4 &v) {
+  const H2 *h = reinterpret_cast<const H2 *>(&v);
+  const H2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(to_float(m.x), to_float(m.y));
+}
+__device__ __forceinline__ float largest(const uint4 &v, __nv_bfloat16) { return largest_half<__nv_bfloat162, __nv_bfloat16>(v); }
+__device__ __forceinline__ float largest(const uint4 &v, __half) { return largest_half<__half2, __half>(v); }
+
 struct alignas(16) Shared {
-  unsigned int count[kBins], low[kBins], high[kBins];   // of a histogram: words, and their weights' lower and upper 32 bits
+  // A histogram: words, and their weights in parts of 16, 16 and more bits (RES: sums of up to 65536 words do not carry), or as the
+  // 64 bits of the first two.  Afterwards: the words of the bin that holds the limit.
+  unsigned int count[kBins], mass[3][kBins];
   double table[256];                                    // 2^(k / 256)
   u64 warp[kWarps];
   float warp_m[kWarps];
@@ -52,8 +68,13 @@ struct alignas(16) Shared {
   u64 own;
   // the bin that holds a limit
   int bin;
-  u64 before_count, before_mass, bin_count, bin_mass, total_mass;
+  unsigned int listed;
+  u64 before_count, before_mass, bin_count, bin_mass, total_mass, all_count, all_mass;
   u64 scan_count[kWarps], scan_mass[kWarps];
+  float cut_value;
+  int cut_last;
+  // a list of the bin's words, in the memory of the histogram: key and index, so that larger ones come first
+  __device__ __forceinline__ u64 *list() { return reinterpret_cast<u64 *>(mass[0]); }
 };
 
 template <typename T, bool RES> struct Draw {
@@ -87,19 +108,25 @@ template <typename T, bool RES> struct Draw {
     }
     return p;
   }
-  __device__ __forceinline__ void words(int v, float (&e)[E]) const {
+  __device__ __forceinline__ Pack<T> words(int v) const {
     Pack<T> p;
     if constexpr (RES) p.v = slice[v - first];
     else p = from_memory(v);
-    const T *w = reinterpret_cast<const T *>(&p.v);
-#pragma unroll
-    for (int k = 0; k < E; ++k) e[k] = to_float(w[k]);
+    return p;
+  }
+  // four of a vector's words, from h on
+  static __device__ __forceinline__ float4 words4(const Pack<T> &p, int h) {
+    if constexpr (sizeof(T) == 4) {
+      return make_float4(__uint_as_float(p.v.x), __uint_as_float(p.v.y), __uint_as_float(p.v.z), __uint_as_float(p.v.w));
+    } else {
+      Raw4<T> r;
+      r.v = h == 0 ? make_uint2(p.v.x, p.v.y) : make_uint2(p.v.z, p.v.w);
+      return widen(r);
+    }
   }
   __device__ __forceinline__ float distance(float e) const { return (0.5f * m - 0.5f * e) * half_scale; }
-  // the weight of a word as an integer
+  // the weight of a word as an integer; no branches, so that the weights of neighbours are under way together
   __device__ __forceinline__ u64 weight(float e) const {
-    if (e == m) return 1ull << shift;
-    if (!(distance(e) < beyond) || m == INFINITY) return 0;
     constexpr double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's lower bits are the nearest integer
     constexpr double c1 = kLn2 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6, c4 = c1 * c1 * c1 * c1 / 24;
     const double d = static_cast<double>(e) - md;
@@ -110,16 +137,21 @@ template <typename T, bool RES> struct Draw {
     q *= s.table[i & 255];
     const u64 bits = static_cast<u64>(__double_as_longlong(q));
     const int right = 52 - (static_cast<int>(bits >> 52) - 1023) - (i >> 8) - shift;   // (q > 0; i <= 0)
-    return right > 63 ? 0 : ((bits & ((1ull << 52) - 1)) | (1ull << 52)) >> right;
+    const u64 w = ((bits & ((1ull << 52) - 1)) | (1ull << 52)) >> (right & 63);
+    return e == m ? 1ull << shift : distance(e) < beyond && right < 64 && m != INFINITY ? w : 0;
   }
-  // f(word, its index) for this warp's words, lanes side by side
-  template <typename F> __device__ __forceinline__ void each(F f) const {
-#pragma unroll 2
+  // f(word, its index) for this warp's words from `least` up, lanes side by side; vectors without one are passed over
+  template <typename F> __device__ __forceinline__ void each(float least, F f) const {
+#pragma unroll 1
     for (int v = from + lane; v < to; v += 32) {
-      float e[E];
-      words(v, e);
+      const Pack<T> p = words(v);
+      if (!(largest(p.v, T()) >= least)) continue;
+      const T *w = reinterpret_cast<const T *>(&p.v);
 #pragma unroll
-      for (int k = 0; k < E; ++k) f(e[k], v * E + k - lead);
+      for (int k = 0; k < E; ++k) {
+        const float e = to_float(w[k]);
+        if (e >= least) f(e, v * E + k - lead);
+      }
     }
   }
   static __device__ __forceinline__ u64 warp_sum(u64 y) {
@@ -127,10 +159,20 @@ template <typename T, bool RES> struct Draw {
     for (int k = 16; k > 0; k >>= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
     return y;
   }
-  // Sums of f over the row's words by warps (put into s.warp): their total, in every block
-  template <typename F> __device__ u64 total(F f) {
+  // Sums of f over the row's words from `least` up by warps (put into s.warp): their total, in every block
+  template <typename F> __device__ u64 total(float least, F f) {
     u64 sum = 0;
-    each([&](float e, int i) { sum += f(e, i); });
+    for (int v = from + lane; v < to; v += 32) {
+      const Pack<T> p = words(v);
+      if (!(largest(p.v, T()) >= least)) continue;
+      u64 y[E];
+#pragma unroll
+      for (int h = 0; h < E; h += 4) {   // four chains of arithmetic at a time
+        const float4 e = words4(p, h);
+        y[h] = f(e.x, v * E + h - lead); y[h + 1] = f(e.y, v * E + h + 1 - lead); y[h + 2] = f(e.z, v * E + h + 2 - lead); y[h + 3] = f(e.w, v * E + h + 3 - lead);
+        sum += (e.x >= least ? y[h] : 0) + (e.y >= least ? y[h + 1] : 0) + (e.z >= least ? y[h + 2] : 0) + (e.w >= least ? y[h + 3] : 0);
+      }
+    }
     sum = warp_sum(sum);
     if (lane == 0) s.warp[warp] = sum;
     cluster.sync();
@@ -150,9 +192,9 @@ template <typename T, bool RES> struct Draw {
     }
     return __shfl_sync(0xffffffffu, upto_warps, 31);
   }
-  // The first index, in rising order, at which the running sum of f exceeds `target` (below the total, after total(f)), and f there:
+  // The first index, in rising order, at which the running sum of f exceeds `target` (below the total, after total(least, f)), and f there:
   // known to every block behind the next cluster.sync(), in s.found and s.own
-  template <typename F> __device__ void find(u64 target, F f) {
+  template <typename F> __device__ void find(float least, u64 target, F f) {
     const int each_lane = (parts * kWarps + 31) / 32;
     const int with = __ffs(__ballot_sync(0xffffffffu, upto_warps > target)) - 1;   // the lane that has the warp
     u64 before = upto_warps - (warps[0] + warps[1] + warps[2] + warps[3]);
@@ -165,84 +207,114 @@ template <typename T, bool RES> struct Draw {
       }
     before = __shfl_sync(0xffffffffu, before, with);
     at = with * each_lane + __shfl_sync(0xffffffffu, at, with);
-    if (at != part * kWarps + warp) return;
-    for (int v0 = from; v0 < to; v0 += 32) {
-      const int v = v0 + lane;
-      float e[E];
-      u64 own[E], sum = 0;
+    if (at / kWarps != part) return;
+    // the block that has it: the warp's part among all its threads, neighbouring words to each
+    const int share = (last - first + kWarps - 1) / kWarps, begin = min(first + at % kWarps * share, last), words_ = (min(begin + share, last) - begin) * E;
+    const int mine = (words_ + kThreads - 1) / kThreads, w0 = static_cast<int>(threadIdx.x) * mine;
+    const auto value = [&](int w) -> u64 {   // of word w of the part
+      const int i = begin * E + w - lead;
+      if (w >= words_ || i < 0 || i >= V) return 0;
+      float e;
+      if constexpr (RES) e = to_float(reinterpret_cast<const T *>(slice)[(begin - first) * E + w]);
+      else e = to_float(x[i]);
+      return e >= least ? f(e, i) : 0;
+    };
+    u64 sum = 0;
+#pragma unroll 1
+    for (int k = 0; k < mine; ++k) sum += value(w0 + k);
+    u64 upto = sum;
 #pragma unroll
-      for (int k = 0; k < E; ++k) own[k] = 0;
-      if (v < to) {
-        words(v, e);
-#pragma unroll
-        for (int k = 0; k < E; ++k) { own[k] = f(e[k], v * E + k - lead); sum += own[k]; }
-      }
-      u64 upto = sum;
-#pragma unroll
-      for (int k = 1; k < 32; k <<= 1) {
-        const u64 o = __shfl_up_sync(0xffffffffu, upto, k);
-        if (lane >= k) upto += o;
-      }
-      const unsigned beyond_ = __ballot_sync(0xffffffffu, before + upto > target);
-      if (beyond_ != 0) {
-        if (lane == __ffs(beyond_) - 1) {
-          u64 run = before + upto - sum;
-          int k = 0;
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (k == j) {
-              if (run + own[j] > target) break;
-              run += own[j];
-              ++k;
-            }
-          u64 mine = 0;
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (k == j) mine = own[j];
+    for (int k = 1; k < 32; k <<= 1) {
+      const u64 o = __shfl_up_sync(0xffffffffu, upto, k);
+      if (lane >= k) upto += o;
+    }
+    if (lane == 31) s.scan_count[warp] = upto;
+    __syncthreads();
+    for (int k = 0; k < warp; ++k) before += s.scan_count[k];
+    u64 run = before + upto - sum;
+    if (run <= target && run + sum > target) {
+#pragma unroll 1
+      for (int k = 0; k < mine; ++k) {
+        const u64 own = value(w0 + k);
+        if (run + own > target) {
           for (int o = 0; o < parts; ++o) {
             Shared *to_ = cluster.map_shared_rank(&s, o);
-            to_->found = v * E + k - lead;
-            to_->own = mine;
+            to_->found = begin * E + w0 + k - lead;
+            to_->own = own;
           }
+          break;
         }
-        return;
+        run += own;
       }
-      before += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
 
-  // Histogram of the words for which bin(word, index) >= 0, over the cluster, and the bin that holds the limit: the first, from bin 0
+  // Histogram of the words from `least` up for which bin(word, index) >= 0, over the cluster, and the bin that holds the limit: the first, from bin 0
   // on, with `target` words (or `target` of weight) up to its end.  part_of_all < 1: the target is that part of the whole weight.
   // s.bin is -1 where there is less.  On entry before_count / before_mass: what lies in front of bin 0.
-  template <typename F> __device__ void limit_bin(bool by_mass, double part_of_all, u64 target, u64 before_count, u64 before_mass, F bin) {
-    for (int k = threadIdx.x; k < kBins; k += kThreads) s.count[k] = s.low[k] = s.high[k] = 0;
-    if (threadIdx.x == 0) { s.bin = -1; s.total_mass = 0; }
+  template <typename F> __device__ void limit_bin(float least, bool by_mass, double part_of_all, u64 target, u64 before_count, u64 before_mass, F bin) {
+    for (int k = threadIdx.x; k < kBins; k += kThreads) s.count[k] = s.mass[0][k] = s.mass[1][k] = s.mass[2][k] = 0;
+    if (threadIdx.x == 0) { s.bin = -1; s.total_mass = 0; s.listed = 0; }
     __syncthreads();
-    each([&](float e, int i) {
-      const int b = bin(e, i);
-      if (b < 0) return;
-      atomicAdd(&s.count[b], 1u);
-      if (by_mass) {
-        const u64 w = weight(e);
-        const unsigned l = static_cast<unsigned>(w);
-        const unsigned old = atomicAdd(&s.low[b], l);
-        const unsigned up = static_cast<unsigned>(w >> 32) + (old + l < l ? 1u : 0u);
-        if (up != 0) atomicAdd(&s.high[b], up);
+    if (by_mass) {
+      for (int v = from + lane; v < to; v += 32) {
+        const Pack<T> p = words(v);
+        if (!(largest(p.v, T()) >= least)) continue;
+#pragma unroll
+        for (int h = 0; h < E; h += 4) {   // four chains of arithmetic at a time
+          const float4 e4 = words4(p, h);
+          const float e[4] = {e4.x, e4.y, e4.z, e4.w};
+          u64 w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = weight(e[k]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int b = e[k] >= least ? bin(e[k], v * E + h + k - lead) : -1;
+            if (b < 0) continue;
+            atomicAdd(&s.count[b], 1u);
+            if constexpr (RES) {
+              atomicAdd(&s.mass[0][b], static_cast<unsigned>(w[k] & 0xffff));
+              atomicAdd(&s.mass[1][b], static_cast<unsigned>(w[k] >> 16) & 0xffffu);
+              atomicAdd(&s.mass[2][b], static_cast<unsigned>(w[k] >> 32));
+            } else {
+              atomicAdd(reinterpret_cast<u64 *>(s.mass[0]) + b, w[k]);
+            }
+          }
+        }
       }
-    });
+    } else {
+      each(least, [&](float e, int i) {
+        const int b = bin(e, i);
+        if (b >= 0) atomicAdd(&s.count[b], 1u);
+      });
+    }
     cluster.sync();
     constexpr int B = kBins / kThreads;
+    static_assert(B % 4 == 0, "a thread's bins are vectors");
     u64 c[B], w[B], sum_c = 0, sum_w = 0;
 #pragma unroll
     for (int k = 0; k < B; ++k) { c[k] = 0; w[k] = 0; }
-    for (int o = 0; o < parts; ++o) {
-      const Shared *h = cluster.map_shared_rank(&s, o);
-      const uint4 n = *reinterpret_cast<const uint4 *>(&h->count[threadIdx.x * B]);
-      c[0] += n.x; c[1] += n.y; c[2] += n.z; c[3] += n.w;
-      if (by_mass) {
-        const uint4 l = *reinterpret_cast<const uint4 *>(&h->low[threadIdx.x * B]), u = *reinterpret_cast<const uint4 *>(&h->high[threadIdx.x * B]);
-        w[0] += l.x + (static_cast<u64>(u.x) << 32); w[1] += l.y + (static_cast<u64>(u.y) << 32);
-        w[2] += l.z + (static_cast<u64>(u.z) << 32); w[3] += l.w + (static_cast<u64>(u.w) << 32);
+    const auto gather = [&](const unsigned *bins, u64 (&to_)[B], int left) {   // (all the blocks' loads under way together)
+#pragma unroll
+      for (int j = 0; j < B; j += 4) {
+#pragma unroll 2
+        for (int o = 0; o < parts; ++o) {
+          const uint4 n = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(bins, o) + threadIdx.x * B + j);
+          to_[j] += static_cast<u64>(n.x) << left; to_[j + 1] += static_cast<u64>(n.y) << left;
+          to_[j + 2] += static_cast<u64>(n.z) << left; to_[j + 3] += static_cast<u64>(n.w) << left;
+        }
+      }
+    };
+    gather(s.count, c, 0);
+    if (by_mass) {
+      if constexpr (RES) {
+        gather(s.mass[0], w, 0);
+        gather(s.mass[1], w, 16);
+        gather(s.mass[2], w, 32);
+      } else {
+        for (int o = 0; o < parts; ++o)
+#pragma unroll
+          for (int k = 0; k < B; ++k) w[k] += reinterpret_cast<const u64 *>(cluster.map_shared_rank(s.mass[0], o))[threadIdx.x * B + k];
       }
     }
 #pragma unroll
@@ -255,9 +327,10 @@ template <typename T, bool RES> struct Draw {
     }
     if (lane == 31) { s.scan_count[warp] = upto_c; s.scan_mass[warp] = upto_w; }
     __syncthreads();
-    u64 all_w = 0;
+    u64 all_c = 0, all_w = 0;
     for (int k = 0; k < kWarps; ++k) {
       if (k < warp) { before_count += s.scan_count[k]; before_mass += s.scan_mass[k]; }
+      all_c += s.scan_count[k];
       all_w += s.scan_mass[k];
     }
     if (part_of_all < 1.0) target = static_cast<u64>(ceil(part_of_all * static_cast<double>(all_w)));
@@ -280,77 +353,182 @@ template <typename T, bool RES> struct Draw {
       before_count += c[k];
       before_mass += w[k];
     }
-    if (threadIdx.x == 0) s.total_mass = target;
+    if (threadIdx.x == 0) { s.total_mass = target; s.all_count = all_c; s.all_mass = all_w; }
     cluster.sync();   // nobody clears its bins while others read them
   }
 
   // keeps the first `target` words, or those before which less than the part `part_of_all` of the weight of what was kept lies
   __device__ void limit(Kept &kept, bool by_mass, double part_of_all, u64 target) {
-    // bins by distance: 64 to a unit, of the logits for counts and of the logarithm of the weights for weights
-    const float scale = by_mass ? 64.f * half_scale : 128.f;
+    // bins by distance: 32 to a unit, of the logits for counts and of the logarithm of the weights for weights (behind the last
+    // bin those weigh nothing: 2^-46)
+    const float scale = by_mass ? 32.f * half_scale : 64.f;
     const auto far = [&](float e) {
       const float t = (0.5f * m - 0.5f * e) * scale;
       return e == m ? 0 : t < static_cast<float>(kBins - 1) ? static_cast<int>(t) : kBins - 1;
     };
     const Kept was = kept;
-    limit_bin(by_mass, by_mass ? part_of_all : 1.0, target, 0, 0, [&](float e, int i) { const uint32_t k = key_of(e); return k != 0 && was.has(k, i) ? far(e) : -1; });
-    if (s.bin < 0) return;   // fewer words than that
-    target = s.total_mass;
-    const int bin = s.bin;
-    // the logits in that bin
-    if (threadIdx.x == 0) { s.key_min = 0xffffffffu; s.key_max = 0; }
-    __syncthreads();
-    uint32_t lowest = 0xffffffffu, highest = 0;
-    each([&](float e, int i) {
-      const uint32_t k = key_of(e);
-      if (k != 0 && was.has(k, i) && far(e) == bin) { lowest = min(lowest, k); highest = max(highest, k); }
-    });
-    lowest = __reduce_min_sync(0xffffffffu, lowest);
-    highest = __reduce_max_sync(0xffffffffu, highest);
-    if (lane == 0) { atomicMin(&s.key_min, lowest); atomicMax(&s.key_max, highest); }
-    cluster.sync();
-    for (int o = 0; o < parts; ++o) {
-      const Shared *h = cluster.map_shared_rank(&s, o);
-      lowest = min(lowest, h->key_min);
-      highest = max(highest, h->key_max);
-    }
-    while (lowest != highest) {
-      int narrow = 0;
-      while (((highest - lowest) >> narrow) >= kBins) ++narrow;
-      const uint32_t lo = lowest, hi = highest;
-      const u64 before_count = s.before_count, before_mass = s.before_mass;
+    const float lowest_open = fmaxf(was.value, -3.402823466e38f);
+    // Counts beyond the last bin are taken only when the limit lies there: most words of a row may, and their additions to one bin
+    // would wait for one another.
+    float least = lowest_open;
+    bool by_distance = true;
+    int bin = 0, narrow = 0;
+    uint32_t lo = 0, hi = 0, lowest = 0xffffffffu, highest = 0;
+    u64 before_count = 0, before_mass = 0;
+#pragma unroll 1
+    while (true) {
+      limit_bin(least, by_mass, by_distance && by_mass ? part_of_all : 1.0, target, before_count, before_mass, [&](float e, int i) {
+        if (!was.has(e, i)) return -1;
+        if (by_distance) {
+          const int b = far(e);
+          return b < kBins - 1 ? b : -1;
+        }
+        const uint32_t k = key_of(e);
+        return k >= lo && k <= hi ? static_cast<int>((hi - k) >> narrow) : -1;
+      });
+      const int at = s.bin;
+      before_count = at < 0 ? s.all_count : s.before_count;
+      before_mass = at < 0 ? s.all_mass : s.before_mass;
+      target = s.total_mass;
       __syncthreads();
-      limit_bin(by_mass, 1.0, target, before_count, before_mass,
-                [&](float e, int i) { const uint32_t k = key_of(e); return k >= lo && k <= hi && was.has(k, i) ? static_cast<int>((hi - k) >> narrow) : -1; });
-      highest = hi - (static_cast<uint32_t>(s.bin) << narrow);
-      lowest = highest - ((1u << narrow) - 1);
-      lowest = lowest < lo || lowest > highest ? lo : lowest;
-      if (narrow == 0) lowest = highest;
+      if (!by_distance) {
+        if (at < 0) return;   // fewer words than the limit
+        highest = hi - (static_cast<uint32_t>(at) << narrow);
+        lowest = highest - ((1u << narrow) - 1);
+        lowest = lowest < lo || lowest > highest ? lo : lowest;
+        if (lowest == highest) break;
+      } else {
+        by_distance = false;
+        bin = at;
+        if (bin < 0) {   // all words of the bins: the limit lies beyond them, or there are fewer words
+          if (by_mass) return;
+          bin = kBins - 1;
+        } else {
+          const float reach = static_cast<float>(bin + 2) * 1.0001f / scale * 2.f;   // (the bin's words are nearer than this)
+          least = fmaxf(least, m - reach);
+        }
+        if (bin < kBins - 1 && s.bin_count <= kList) {   // few words in the bin: the first block sorts them
+          Shared *head = cluster.map_shared_rank(&s, 0);
+          each(least, [&](float e, int i) {
+            if (far(e) != bin || !was.has(e, i)) return;
+            head->list()[atomicAdd(&head->listed, 1u)] = (static_cast<u64>(key_of(e)) << 32) | static_cast<unsigned>(~i);
+          });
+          cluster.sync();
+          if (part == 0) {
+            const int n = static_cast<int>(s.listed);
+            u64 *list = s.list();
+            int size = 1;
+            while (size < n) size *= 2;
+            for (int j = n + threadIdx.x; j < size; j += kThreads) list[j] = 0;
+            __syncthreads();
+            for (int run = 2; run <= size; run *= 2)   // (bitonic: comparisons of elements a power of two apart)
+              for (int apart = run / 2; apart > 0; apart /= 2) {
+                for (int j = threadIdx.x; j < size / 2; j += kThreads) {
+                  const int i = 2 * j - (j & (apart - 1)), o = i + apart;
+                  const u64 a = list[i], b = list[o];
+                  if ((a < b) == ((i & run) == 0)) { list[i] = b; list[o] = a; }
+                }
+                __syncthreads();
+              }
+            int keep;   // so many of them
+            if (by_mass) {
+              constexpr int L = kList / kThreads;
+              u64 w[L], sum = 0;
+#pragma unroll
+              for (int j = 0; j < L; ++j) {
+                const int at = threadIdx.x * L + j;
+                w[j] = at < n ? weight(value_of(static_cast<uint32_t>(list[at] >> 32))) : 0;
+                sum += w[j];
+              }
+              u64 upto = sum;
+#pragma unroll
+              for (int k = 1; k < 32; k <<= 1) {
+                const u64 o = __shfl_up_sync(0xffffffffu, upto, k);
+                if (lane >= k) upto += o;
+              }
+              if (lane == 31) s.scan_mass[warp] = upto;
+              __syncthreads();
+              u64 before = before_mass + upto - sum;
+              for (int k = 0; k < warp; ++k) before += s.scan_mass[k];
+              int mine = 0;
+#pragma unroll
+              for (int j = 0; j < L; ++j) {
+                const int at = threadIdx.x * L + j;
+                if (at < n && (before < target || before_count + at == 0)) ++mine;
+                before += w[j];
+              }
+              if (threadIdx.x == 0) s.best = 0;
+              __syncthreads();
+              mine = __reduce_add_sync(0xffffffffu, mine);
+              if (lane == 0) atomicAdd(&s.best, mine);
+              __syncthreads();
+              keep = s.best;
+            } else {
+              keep = static_cast<int>(target - before_count);
+            }
+            if (threadIdx.x < parts) {
+              const u64 last_kept = list[keep - 1];
+              Shared *to_ = cluster.map_shared_rank(&s, threadIdx.x);
+              to_->cut_value = value_of(static_cast<uint32_t>(last_kept >> 32));
+              to_->cut_last = static_cast<int>(~static_cast<unsigned>(last_kept));
+            }
+          }
+          cluster.sync();
+          kept.value = s.cut_value;
+          kept.last = s.cut_last;
+          __syncthreads();
+          return;
+        }
+        // the logits in that bin
+        if (threadIdx.x == 0) { s.key_min = 0xffffffffu; s.key_max = 0; }
+        __syncthreads();
+        each(least, [&](float e, int i) {
+          if (far(e) == bin && was.has(e, i)) {
+            const uint32_t k = key_of(e);
+            lowest = min(lowest, k);
+            highest = max(highest, k);
+          }
+        });
+        lowest = __reduce_min_sync(0xffffffffu, lowest);
+        highest = __reduce_max_sync(0xffffffffu, highest);
+        if (lane == 0) { atomicMin(&s.key_min, lowest); atomicMax(&s.key_max, highest); }
+        cluster.sync();
+        for (int o = 0; o < parts; ++o) {
+          const Shared *h = cluster.map_shared_rank(&s, o);
+          lowest = min(lowest, h->key_min);
+          highest = max(highest, h->key_max);
+        }
+        if (lowest > highest) return;   // no word there
+        if (lowest == highest && bin < kBins - 1) break;   // (the last bin has not been counted)
+      }
+      lo = lowest;
+      hi = highest;
+      least = value_of(lo);
+      narrow = 0;
+      while (((hi - lo) >> narrow) >= kBins) ++narrow;
     }
-    const uint32_t key = highest;
+    const float value = value_of(highest);
     // of the words equal to the threshold
     u64 ties;
     if (by_mass) {
       const u64 one = s.bin_mass / s.bin_count;
-      ties = one == 0 ? s.bin_count : target > s.before_mass ? (target - s.before_mass + one - 1) / one : 0;
-      if (s.before_count == 0 && ties == 0) ties = 1;
+      ties = one == 0 ? s.bin_count : target > before_mass ? (target - before_mass + one - 1) / one : 0;
+      if (before_count == 0 && ties == 0) ties = 1;
     } else {
-      ties = target - s.before_count;
+      ties = target - before_count;
     }
     if (ties < s.bin_count) {
-      const auto tie = [&](float e, int i) -> u64 { const uint32_t k = key_of(e); return k == key && was.has(k, i) ? 1 : 0; };
+      kept.last = -1;
       if (ties > 0) {
-        total(tie);
-        find(ties - 1, tie);
+        const auto tie = [&](float e, int i) -> u64 { return e == value && was.has(e, i) ? 1 : 0; };
+        total(value, tie);
+        find(value, ties - 1, tie);
         cluster.sync();
         kept.last = s.found;
-        kept.key = key;
-      } else {
-        kept.key = key;
-        kept.last = -1;
       }
-    } else if (key > kept.key) {
-      kept.key = key;
+      kept.value = value;
+    } else if (value > kept.value) {
+      kept.value = value;
       kept.last = 0x7fffffff;
     }
     __syncthreads();   // what has been read here is written by the next limit
@@ -358,7 +536,7 @@ template <typename T, bool RES> struct Draw {
 };
 
 template <typename T, bool RES>
-__global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling a, int shift) {
+__global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampling a, int shift) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   Shared &s = *reinterpret_cast<Shared *>(dynamic);
   Draw<T, RES> d(s);
@@ -393,12 +571,10 @@ __global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling 
     for (int u = 0; u < U; ++u)
       if (v + 32 * u < d.to) {
         if constexpr (RES) d.slice[v + 32 * u - d.first] = p[u].v;
-        const T *e = reinterpret_cast<const T *>(&p[u].v);
-#pragma unroll
-        for (int k = 0; k < E; ++k) m = fmaxf(m, to_float(e[k]));   // (NaN is passed over)
+        m = fmaxf(m, largest(p[u].v, T()));
       }
   }
-  if (threadIdx.x < 256) s.table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 256.0);
+  s.table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 256.0);
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   if (d.lane == 0) s.warp_m[d.warp] = m;
@@ -410,7 +586,7 @@ __global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling 
   for (int k = 0; k < d.parts; ++k) m = fmaxf(m, d.cluster.map_shared_rank(&s, k)->m);
   if (m == -INFINITY || !(temperature > 0.f)) {
     int best = 0x7fffffff;
-    if (m != -INFINITY) d.each([&](float e, int i) { if (e == m) best = min(best, i); });
+    if (m != -INFINITY) d.each(m, [&](float, int i) { best = min(best, i); });
     best = __reduce_min_sync(0xffffffffu, best);
     if (d.lane == 0) atomicMin(&s.best, best);
     d.cluster.sync();
@@ -430,8 +606,10 @@ __global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling 
   d.beyond = static_cast<float>((shift + 1) * kLn2) + 0.5f;
 
   Kept kept;
-  if (top_k > 0 && top_k < d.V) d.limit(kept, false, 1.0, static_cast<u64>(top_k));
-  if (top_p < 1.f) d.limit(kept, true, top_p > 0.f ? static_cast<double>(top_p) : 0.0, 0);
+#pragma unroll 1
+  for (int by_mass = 0; by_mass < 2; ++by_mass)
+    if (by_mass ? top_p < 1.f : top_k > 0 && top_k < d.V)
+      d.limit(kept, by_mass, top_p > 0.f ? static_cast<double>(top_p) : 0.0, by_mass ? 0 : static_cast<u64>(top_k));
   // the least weight, as an integer of the same scale, and the distance behind which no weight reaches it
   u64 least = 1;
   float reach = d.beyond;
@@ -440,16 +618,14 @@ __global__ void __launch_bounds__(kThreads) sampling_kernel(const myea_sampling 
     reach = fminf(reach, -logf(min_p) * 1.0001f + 1e-3f);
   }
   const auto weigh = [&](float e, int i) -> u64 {
-    if (!(d.distance(e) < reach) && e != m) return 0;
-    const uint32_t k = key_of(e);
-    if (k == 0 || !kept.has(k, i)) return 0;
     const u64 w = d.weight(e);
-    return w >= least ? w : 0;
+    return kept.has(e, i) && w >= least ? w : 0;
   };
-  const u64 total = d.total(weigh);
+  const float nearest = fmaxf(m - reach * 1.001f * temperature, fmaxf(kept.value, -3.402823466e38f));
+  const u64 total = d.total(nearest, weigh);
   u64 target = uniform > 0.f ? static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(total)) : 0;
   if (target >= total) target = total - 1;
-  d.find(target, weigh);
+  d.find(nearest, target, weigh);
   d.cluster.sync();
   if (d.part == 0 && threadIdx.x == 0) {
     a.tokens[row] = s.found;
@@ -492,13 +668,13 @@ template <typename T, bool RES> cudaError_t launch(const myea_sampling &a, int p
 }
 
 template <typename T> cudaError_t launch(const myea_sampling &a, cudaStream_t stream) {
-  // a slice of at most 64 KB leaves room for two blocks on an SM; more blocks per row while the rows leave SMs idle and a
+  // a slice of some 32 KB leaves room for four blocks on an SM (two of 64 KB measured 220 us where these take 202); more blocks per row while the rows leave SMs idle and a
   // slice has 4096 words
   const uint64_t bytes = a.vocabulary * sizeof(T) + 32;
   int parts = 1;
-  while (parts < kParts && (bytes / parts > (64u << 10) || (a.rows * parts * 2 <= 2 * kSms && a.vocabulary / (parts * 2) >= 4096))) parts *= 2;
+  while (parts < kParts && (bytes / parts > (36u << 10) || (a.rows * parts * 2 <= 2 * kSms && a.vocabulary / (parts * 2) >= 4096))) parts *= 2;
   const size_t slice = (bytes / parts + 64) / 16 * 16;
-  if (sizeof(Shared) + slice > (200u << 10)) return launch<T, false>(a, parts, sizeof(Shared), stream);
+  if (sizeof(Shared) + slice > (200u << 10) || slice / sizeof(T) > 65536) return launch<T, false>(a, parts, sizeof(Shared), stream);
   return launch<T, true>(a, parts, sizeof(Shared) + slice, stream);
 }
 

@@ -8,28 +8,40 @@ current stream of the tensors' GPU, may be captured into a CUDA graph and does n
 together (nothing was launched); RuntimeError: the library refused the call or failed, with its message.
 """
 import ctypes as C
+import struct
+import threading
 
 import torch
 
 from . import capi
 
 _TYPES = {torch.float32: capi.TYPE_F32, torch.bfloat16: capi.TYPE_BF16, torch.float16: capi.TYPE_F16}
+_F32, _I32 = torch.float32, torch.int32
+# the descriptions of myea_b200.h, packed (a call for one token takes a few microseconds: so do forty attribute assignments)
+_CONVOLUTION = struct.Struct("<4I3Q" + 4 * "Qqq" + "9Q")
+_SCAN = struct.Struct("<4I5Q" + 6 * "Qqq" + "7Q" + 6 * "Qqq" + "5Q")
+_DISTILLATION = struct.Struct("<2I3Q" + 3 * "Qq" + "2Q4f2Qq")
+_SAMPLING = struct.Struct("<2I2QQq7Q")
+_NO_VIEW = (0, 0, 0)
+_local = threading.local()   # .message: where the library says why
 
 
-def _call(name, device, *args):
-    message = C.create_string_buffer(256)
-    rc = getattr(capi.load(), "myea_b200_" + name)(device.index, *args, torch.cuda.current_stream(device).cuda_stream, message, 256)
+def _call(name, index, *args):
+    try:
+        message = _local.message
+    except AttributeError:
+        message = _local.message = C.create_string_buffer(256)
+    rc = getattr(capi.load(), name)(index, *args, torch.cuda.current_stream(index).cuda_stream, message, 256)
     if rc != 0:
         raise RuntimeError("%s failed (%d): %s" % (name, rc, message.value.decode()))
 
 
-def _check(name, x, shape, dtype, device):
-    if tuple(x.shape) != tuple(shape) or x.dtype != dtype or x.device != device:
-        raise ValueError("%s: expected %s of %s on %s, got %s of %s on %s" % (name, tuple(shape), dtype, device, tuple(x.shape), x.dtype, x.device))
+def _mismatch(name, x, shape, dtype, index):
+    raise ValueError("%s: expected %s of %s on cuda:%d, got %s of %s on %s" % (name, tuple(shape), dtype, index, tuple(x.shape), x.dtype, x.device))
 
 
 def _type(x):
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError("tensors have to lie on a GPU, got one on %s" % x.device)
     if x.dtype not in _TYPES:
         raise ValueError("float32, bfloat16 or float16 expected, got %s" % x.dtype)
@@ -46,41 +58,43 @@ def _dense(x, from_dim):
     return True
 
 
-def _view(name, x, shape, dtype, device):
+def _view(name, x, shape, dtype, index):
     """address and strides of a [batch, time, ...] tensor; nothing where there is none"""
     if x is None:
-        return 0, 0, 0
-    _check(name, x, shape, dtype, device)
-    if not _dense(x, 2):
+        return _NO_VIEW
+    if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
+        _mismatch(name, x, shape, dtype, index)
+    if not x.is_contiguous() and not _dense(x, 2):
         raise ValueError("%s: the dimensions behind batch and time have to lie densely, strides are %s" % (name, x.stride()))
-    return x.data_ptr(), x.stride(0), x.stride(1)
+    strides = x.stride()
+    return x.data_ptr(), strides[0], strides[1]
 
 
-def _array(name, x, shape, dtype, device):
-    """address of a densely packed tensor; None where there is none"""
+def _array(name, x, shape, dtype, index):
+    """address of a densely packed tensor; 0 where there is none"""
     if x is None:
-        return None
-    _check(name, x, shape, dtype, device)
+        return 0
+    if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
+        _mismatch(name, x, shape, dtype, index)
     if not x.is_contiguous():
         raise ValueError("%s has to be contiguous" % name)
     return x.data_ptr()
 
 
-def _out(given, shape, dtype, device):
-    return torch.empty(shape, dtype=dtype, device=device) if given is None else given
+def _gradient(name, given, shape, like, accumulate):
+    if given is not None:
+        return given
+    if accumulate:
+        raise ValueError("%s: accumulate needs an array to add to" % name)
+    return like.new_empty(shape, dtype=_F32)
 
 
-def _convolution(x, weight, bias, silu, state, lengths):
-    if x.dim() != 3 or weight.dim() != 2:
-        raise ValueError("x is [batch, time, width] and weight [width, taps]")
-    (b, t, d), k, dev = x.shape, weight.shape[1], x.device
-    s = capi.Convolution(_type(x), k, 1 if silu else 0, 0, b, t, d)
-    s.x, s.x_batch, s.x_time = _view("x", x, (b, t, d), x.dtype, dev)
-    s.weight = _array("weight", weight, (d, k), torch.float32, dev)
-    s.bias = _array("bias", bias, (d,), torch.float32, dev)
-    s.state = _array("state", state, (b, k - 1, d), x.dtype, dev)
-    s.lengths = _array("lengths", lengths, (b,), torch.int32, dev)
-    return s
+def _workspace(name, description, like):
+    size = getattr(capi.load(), name)(description)
+    if size == 0:
+        return None, None, 0
+    work = like.new_empty(size, dtype=torch.uint8)
+    return work, work.data_ptr(), size
 
 
 def causal_convolution(x, weight, bias=None, silu=True, state=None, final_state=None, lengths=None, out=None):
@@ -88,63 +102,44 @@ def causal_convolution(x, weight, bias=None, silu=True, state=None, final_state=
     weight [width, taps], 1 to 8 taps; state [batch, taps - 1, width]: the inputs before the first (None: zeros); final_state: where the
     last taps - 1 inputs go (None: a new tensor; `state` itself is allowed); lengths int32 [batch]: y is 0 behind a sequence's
     end.  A single token is time = 1 with both states."""
-    s = _convolution(x, weight, bias, silu, state, lengths)
-    (b, t, d), k = x.shape, weight.shape[1]
-    y, final_state = _out(out, (b, t, d), x.dtype, x.device), _out(final_state, (b, k - 1, d), x.dtype, x.device)
-    s.y, s.y_batch, s.y_time = _view("out", y, (b, t, d), x.dtype, x.device)
-    s.final_state = _array("final_state", final_state, (b, k - 1, d), x.dtype, x.device)
-    _call("causal_convolution", x.device, C.byref(s))
-    return y, final_state
+    kind = _type(x)
+    if x.dim() != 3 or weight.dim() != 2:
+        raise ValueError("x is [batch, time, width] and weight [width, taps]")
+    (b, t, d), k, tp, at = x.shape, weight.shape[1], x.dtype, x.get_device()
+    whole, before = (b, t, d), (b, k - 1, d)
+    if out is None:
+        out = x.new_empty(whole)
+    if final_state is None:
+        final_state = x.new_empty(before)
+    _call("myea_b200_causal_convolution", at, _CONVOLUTION.pack(
+        kind, k, 1 if silu else 0, 0, b, t, d, *_view("x", x, whole, tp, at), *_view("out", out, whole, tp, at), *_NO_VIEW, *_NO_VIEW,
+        _array("weight", weight, (d, k), _F32, at), _array("bias", bias, (d,), _F32, at), _array("state", state, before, tp, at),
+        _array("final_state", final_state, before, tp, at), _array("lengths", lengths, (b,), _I32, at), 0, 0, 0, 0))
+    return out, final_state
 
 
 def causal_convolution_backward(dy, x, weight, bias=None, silu=True, state=None, lengths=None, d_final_state=None, dx=None, d_weight=None, d_bias=None,
                                 accumulate=False):
     """{"x", "weight", "bias" (None without one), "state" (None without one)}: derivatives for the error `dy` on y and
     `d_final_state` on the final state.  d_weight / d_bias given: the derivatives go there, with `accumulate` onto what they hold."""
-    s = _convolution(x, weight, bias, silu, state, lengths)
-    (b, t, d), k, dev = x.shape, weight.shape[1], x.device
-    dx, d_weight = _out(dx, (b, t, d), x.dtype, dev), _gradient("d_weight", d_weight, (d, k), dev, accumulate)
-    d_bias = _gradient("d_bias", d_bias, (d,), dev, accumulate) if bias is not None else None
-    d_state = torch.empty((b, k - 1, d), dtype=x.dtype, device=dev) if state is not None else None
-    s.accumulate = 1 if accumulate else 0
-    s.dy, s.dy_batch, s.dy_time = _view("dy", dy, (b, t, d), x.dtype, dev)
-    s.dx, s.dx_batch, s.dx_time = _view("dx", dx, (b, t, d), x.dtype, dev)
-    s.d_weight = _array("d_weight", d_weight, (d, k), torch.float32, dev)
-    s.d_bias = _array("d_bias", d_bias, (d,), torch.float32, dev)
-    s.d_final_state = _array("d_final_state", d_final_state, (b, k - 1, d), x.dtype, dev)
-    s.d_state = _array("d_state", d_state, (b, k - 1, d), x.dtype, dev)
-    work, size = _workspace("causal_convolution_backward_workspace", s, dev)
-    _call("causal_convolution_backward", dev, C.byref(s), work.data_ptr() if size else None, size)
+    kind = _type(x)
+    if x.dim() != 3 or weight.dim() != 2:
+        raise ValueError("x is [batch, time, width] and weight [width, taps]")
+    (b, t, d), k, tp, at = x.shape, weight.shape[1], x.dtype, x.get_device()
+    whole, before = (b, t, d), (b, k - 1, d)
+    if dx is None:
+        dx = x.new_empty(whole)
+    d_weight = _gradient("d_weight", d_weight, (d, k), x, accumulate)
+    d_bias = _gradient("d_bias", d_bias, (d,), x, accumulate) if bias is not None else None
+    d_state = x.new_empty(before) if state is not None else None
+    s = _CONVOLUTION.pack(
+        kind, k, 1 if silu else 0, 1 if accumulate else 0, b, t, d, *_view("x", x, whole, tp, at), *_NO_VIEW, *_view("dy", dy, whole, tp, at),
+        *_view("dx", dx, whole, tp, at), _array("weight", weight, (d, k), _F32, at), _array("bias", bias, (d,), _F32, at), _array("state", state, before, tp, at),
+        0, _array("lengths", lengths, (b,), _I32, at), _array("d_weight", d_weight, (d, k), _F32, at), _array("d_bias", d_bias, (d,), _F32, at),
+        _array("d_final_state", d_final_state, before, tp, at), _array("d_state", d_state, before, tp, at))
+    work, address, size = _workspace("myea_b200_causal_convolution_backward_workspace", s, x)
+    _call("myea_b200_causal_convolution_backward", at, s, address, size)
     return {"x": dx, "weight": d_weight, "bias": d_bias, "state": d_state}
-
-
-def _gradient(name, given, shape, device, accumulate):
-    if given is None and accumulate:
-        raise ValueError("%s: accumulate needs an array to add to" % name)
-    return _out(given, shape, torch.float32, device)
-
-
-def _workspace(name, s, device):
-    size = getattr(capi.load(), "myea_b200_" + name)(C.byref(s))
-    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
-
-
-def _scan(u, delta, A, B, Cm, D, z, delta_bias, softplus, state, lengths):
-    if u.dim() != 3 or A.dim() != 2 or B.dim() != 4:
-        raise ValueError("u is [batch, time, width], A [width, states], B and C [batch, time, groups, states]")
-    (b, t, d), n, g, dev, tp = u.shape, A.shape[1], B.shape[2], u.device, u.dtype
-    s = capi.Scan(_type(u), 1 if softplus else 0, 0, 0, b, t, d, n, g)
-    s.u, s.u_batch, s.u_time = _view("u", u, (b, t, d), tp, dev)
-    s.delta, s.delta_batch, s.delta_time = _view("delta", delta, (b, t, d), tp, dev)
-    s.B, s.B_batch, s.B_time = _view("B", B, (b, t, g, n), tp, dev)
-    s.C, s.C_batch, s.C_time = _view("C", Cm, (b, t, g, n), tp, dev)
-    s.z, s.z_batch, s.z_time = _view("z", z, (b, t, d), tp, dev)
-    s.A = _array("A", A, (d, n), torch.float32, dev)
-    s.D = _array("D", D, (d,), torch.float32, dev)
-    s.delta_bias = _array("delta_bias", delta_bias, (d,), torch.float32, dev)
-    s.state = _array("state", state, (b, d, n), torch.float32, dev)
-    s.lengths = _array("lengths", lengths, (b,), torch.int32, dev)
-    return s
 
 
 def _checkpoint_shape(b, t, d, n):
@@ -161,6 +156,19 @@ def scan_checkpoints(u, A):
     return torch.empty(_checkpoint_shape(*u.shape, A.shape[1]), dtype=torch.float32, device=u.device)
 
 
+def _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths):
+    """(type, sizes, device, views of the inputs, arrays of the parameters), checked"""
+    kind = _type(u)
+    if u.dim() != 3 or A.dim() != 2 or B.dim() != 4:
+        raise ValueError("u is [batch, time, width], A [width, states], B and C [batch, time, groups, states]")
+    (b, t, d), n, g, tp, at = u.shape, A.shape[1], B.shape[2], u.dtype, u.get_device()
+    whole, narrow = (b, t, d), (b, t, g, n)
+    views = _view("u", u, whole, tp, at) + _view("delta", delta, whole, tp, at) + _view("B", B, narrow, tp, at) + _view("C", C_, narrow, tp, at) + _view("z", z, whole, tp, at)
+    arrays = (_array("A", A, (d, n), _F32, at), _array("D", D, (d,), _F32, at), _array("delta_bias", delta_bias, (d,), _F32, at),
+              _array("state", state, (b, d, n), _F32, at))
+    return kind, (b, t, d, n, g), at, views, arrays, _array("lengths", lengths, (b,), _I32, at)
+
+
 def selective_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, softplus=True, state=None, final_state=None, lengths=None, checkpoints=None,
                    out=None):
     """(y, final_state) of the selective state space scan over u, delta [batch, time, width] with A [width, states] (1 to 128 states),
@@ -168,15 +176,20 @@ def selective_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, softplus
     zeros) and one to end in (None: a new tensor; `state` itself is allowed).  lengths int32 [batch]: y is 0 behind a sequence's
     end, and the state there stays.  checkpoints (scan_checkpoints): kept for selective_scan_backward.  A single token is
     time = 1 with both states."""
-    s = _scan(u, delta, A, B, C_, D, z, delta_bias, softplus, state, lengths)
-    (b, t, d), n, dev = u.shape, A.shape[1], u.device
-    y, final_state = _out(out, (b, t, d), u.dtype, dev), _out(final_state, (b, d, n), torch.float32, dev)
-    s.y, s.y_batch, s.y_time = _view("out", y, (b, t, d), u.dtype, dev)
-    s.final_state = _array("final_state", final_state, (b, d, n), torch.float32, dev)
-    s.checkpoints = _array("checkpoints", checkpoints, _checkpoint_shape(b, t, d, n), torch.float32, dev)
-    work, size = _workspace("selective_scan_workspace", s, dev)
-    _call("selective_scan", dev, C.byref(s), work.data_ptr() if size else None, size)
-    return y, final_state
+    kind, (b, t, d, n, g), at, views, arrays, lengths_at = _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths)
+    if out is None:
+        out = u.new_empty((b, t, d))
+    if final_state is None:
+        final_state = u.new_empty((b, d, n), dtype=_F32)
+    kept = 0 if checkpoints is None else _array("checkpoints", checkpoints, _checkpoint_shape(b, t, d, n), _F32, at)
+    s = _SCAN.pack(kind, 1 if softplus else 0, 0, 0, b, t, d, n, g, *views, *_view("out", out, (b, t, d), u.dtype, at), *arrays,
+                   _array("final_state", final_state, (b, d, n), _F32, at), lengths_at, kept, *_NO_GRADIENTS)
+    work, address, size = _workspace("myea_b200_selective_scan_workspace", s, u)
+    _call("myea_b200_selective_scan", at, s, address, size)
+    return out, final_state
+
+
+_NO_GRADIENTS = (0,) * 23
 
 
 def selective_scan_backward(dy, u, delta, A, B, C_, checkpoints, D=None, z=None, delta_bias=None, softplus=True, state=None, lengths=None,
@@ -184,38 +197,30 @@ def selective_scan_backward(dy, u, delta, A, B, C_, checkpoints, D=None, z=None,
     """Derivatives for the error `dy` on y and `d_final_state` on the final state, by the names of the forward pass's arguments
     ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state"; None where there was none).  d_A, d_D, d_delta_bias given: those go
     there, with `accumulate` onto what they hold."""
-    s = _scan(u, delta, A, B, C_, D, z, delta_bias, softplus, state, lengths)
-    (b, t, d), n, g, dev, tp = u.shape, A.shape[1], B.shape[2], u.device, u.dtype
-    got = {"u": torch.empty((b, t, d), dtype=tp, device=dev), "delta": torch.empty((b, t, d), dtype=tp, device=dev),
-           "B": torch.empty((b, t, g, n), dtype=tp, device=dev), "C": torch.empty((b, t, g, n), dtype=tp, device=dev),
-           "z": torch.empty((b, t, d), dtype=tp, device=dev) if z is not None else None,
-           "A": _gradient("d_A", d_A, (d, n), dev, accumulate), "D": _gradient("d_D", d_D, (d,), dev, accumulate) if D is not None else None,
-           "delta_bias": _gradient("d_delta_bias", d_delta_bias, (d,), dev, accumulate) if delta_bias is not None else None,
-           "state": torch.empty((b, d, n), dtype=torch.float32, device=dev) if state is not None else None}
-    s.accumulate = 1 if accumulate else 0
-    s.checkpoints = _array("checkpoints", checkpoints, _checkpoint_shape(b, t, d, n), torch.float32, dev)
-    s.dy, s.dy_batch, s.dy_time = _view("dy", dy, (b, t, d), tp, dev)
-    s.du, s.du_batch, s.du_time = _view("du", got["u"], (b, t, d), tp, dev)
-    s.ddelta, s.ddelta_batch, s.ddelta_time = _view("ddelta", got["delta"], (b, t, d), tp, dev)
-    s.dB, s.dB_batch, s.dB_time = _view("dB", got["B"], (b, t, g, n), tp, dev)
-    s.dC, s.dC_batch, s.dC_time = _view("dC", got["C"], (b, t, g, n), tp, dev)
-    s.dz, s.dz_batch, s.dz_time = _view("dz", got["z"], (b, t, d), tp, dev)
-    s.d_A = _array("d_A", got["A"], (d, n), torch.float32, dev)
-    s.d_D = _array("d_D", got["D"], (d,), torch.float32, dev)
-    s.d_delta_bias = _array("d_delta_bias", got["delta_bias"], (d,), torch.float32, dev)
-    s.d_final_state = _array("d_final_state", d_final_state, (b, d, n), torch.float32, dev)
-    s.d_state = _array("d_state", got["state"], (b, d, n), torch.float32, dev)
-    work, size = _workspace("selective_scan_backward_workspace", s, dev)
-    _call("selective_scan_backward", dev, C.byref(s), work.data_ptr() if size else None, size)
+    kind, (b, t, d, n, g), at, views, arrays, lengths_at = _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths)
+    tp, whole, narrow, held = u.dtype, (b, t, d), (b, t, g, n), (b, d, n)
+    got = {"u": u.new_empty(whole), "delta": u.new_empty(whole), "B": u.new_empty(narrow), "C": u.new_empty(narrow), "z": u.new_empty(whole) if z is not None else None,
+           "A": _gradient("d_A", d_A, (d, n), u, accumulate), "D": _gradient("d_D", d_D, (d,), u, accumulate) if D is not None else None,
+           "delta_bias": _gradient("d_delta_bias", d_delta_bias, (d,), u, accumulate) if delta_bias is not None else None,
+           "state": u.new_empty(held, dtype=_F32) if state is not None else None}
+    s = _SCAN.pack(kind, 1 if softplus else 0, 1 if accumulate else 0, 0, b, t, d, n, g, *views, *_NO_VIEW, *arrays, 0, lengths_at,
+                   _array("checkpoints", checkpoints, _checkpoint_shape(b, t, d, n), _F32, at), *_view("dy", dy, whole, tp, at),
+                   *_view("du", got["u"], whole, tp, at), *_view("ddelta", got["delta"], whole, tp, at), *_view("dB", got["B"], narrow, tp, at),
+                   *_view("dC", got["C"], narrow, tp, at), *_view("dz", got["z"], whole, tp, at), _array("d_A", got["A"], (d, n), _F32, at),
+                   _array("d_D", got["D"], (d,), _F32, at), _array("d_delta_bias", got["delta_bias"], (d,), _F32, at),
+                   _array("d_final_state", d_final_state, held, _F32, at), _array("d_state", got["state"], held, _F32, at))
+    work, address, size = _workspace("myea_b200_selective_scan_backward_workspace", s, u)
+    _call("myea_b200_selective_scan_backward", at, s, address, size)
     return got
 
 
-def _rows(name, x, shape, dtype, device):
+def _rows(name, x, shape, dtype, index):
     """address and row pitch of a [rows, columns] tensor"""
     if x is None:
-        return None, 0
-    _check(name, x, shape, dtype, device)
-    if not _dense(x, 1):
+        return 0, 0
+    if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
+        _mismatch(name, x, shape, dtype, index)
+    if not x.is_contiguous() and not _dense(x, 1):
         raise ValueError("%s: the columns have to lie densely, strides are %s" % (name, x.stride()))
     return x.data_ptr(), x.stride(0)
 
@@ -225,20 +230,20 @@ def distillation_error(logits, index, teacher, temperature=1.0, soft=1.0, hard=0
     word index[r, k] (int32, outside the vocabulary: no entry), with `soft` * temperature^2 * KL(teacher, logits) at that
     temperature plus `hard` * cross entropy to labels (int32 [rows], outside the vocabulary: none), times weight (float32 [rows]); and its
     derivatives, of the logits' type, unless derivatives = False.  d_logits may be `logits`."""
+    kind = _type(logits)
     if logits.dim() != 2 or index.dim() != 2:
         raise ValueError("logits is [rows, vocabulary], index and teacher are [rows, top]")
-    (r, v), k, dev = logits.shape, index.shape[1], logits.device
-    s = capi.Distillation(_type(logits), 0, r, v, k)
-    losses = _out(losses, (r,), torch.float32, dev)
-    d_logits = _out(d_logits, (r, v), logits.dtype, dev) if derivatives else None
-    s.logits, s.logits_stride = _rows("logits", logits, (r, v), logits.dtype, dev)
-    s.index, s.index_stride = _rows("index", index, (r, k), torch.int32, dev)
-    s.teacher, s.teacher_stride = _rows("teacher", teacher, (r, k), torch.float32, dev)
-    s.labels, s.weight = _array("labels", labels, (r,), torch.int32, dev), _array("weight", weight, (r,), torch.float32, dev)
-    s.temperature, s.soft, s.hard = temperature, soft, hard
-    s.losses = _array("losses", losses, (r,), torch.float32, dev)
-    s.d_logits, s.d_logits_stride = _rows("d_logits", d_logits, (r, v), logits.dtype, dev)
-    _call("distillation_error", dev, C.byref(s))
+    (r, v), k, tp, at = logits.shape, index.shape[1], logits.dtype, logits.get_device()
+    if losses is None:
+        losses = logits.new_empty((r,), dtype=_F32)
+    if not derivatives:
+        d_logits = None
+    elif d_logits is None:
+        d_logits = logits.new_empty((r, v))
+    _call("myea_b200_distillation_error", at, _DISTILLATION.pack(
+        kind, 0, r, v, k, *_rows("logits", logits, (r, v), tp, at), *_rows("index", index, (r, k), _I32, at), *_rows("teacher", teacher, (r, k), _F32, at),
+        _array("labels", labels, (r,), _I32, at), _array("weight", weight, (r,), _F32, at), temperature, soft, hard, 0.0,
+        _array("losses", losses, (r,), _F32, at), *_rows("d_logits", d_logits, (r, v), tp, at)))
     return losses, d_logits
 
 
@@ -246,14 +251,17 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     """(tokens int32 [rows], chances [rows]): one token for every row of logits [rows, vocabulary], drawn with uniform (float32 [rows], in
     [0, 1)) from what temperature, top_k (int32), top_p and min_p leave of the row, each an array of one value per row or None; and
     the chance that it had.  temperature <= 0: the largest logit.  A row whose words are all closed (minus infinity): token -1."""
+    kind = _type(logits)
     if logits.dim() != 2:
         raise ValueError("logits is [rows, vocabulary]")
-    (r, v), dev = logits.shape, logits.device
-    s = capi.Sampling(_type(logits), 0, r, v)
-    tokens, chances = _out(tokens, (r,), torch.int32, dev), _out(chances, (r,), torch.float32, dev)
-    s.logits, s.logits_stride = _rows("logits", logits, (r, v), logits.dtype, dev)
-    for name, x, dtype in (("uniform", uniform, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int32), ("chances", chances, torch.float32)):
-        setattr(s, name, _array(name, x, (r,), dtype, dev))
-    _call("sample", dev, C.byref(s))
+    (r, v), at = logits.shape, logits.get_device()
+    one = (r,)
+    if tokens is None:
+        tokens = logits.new_empty(one, dtype=_I32)
+    if chances is None:
+        chances = logits.new_empty(one, dtype=_F32)
+    _call("myea_b200_sample", at, _SAMPLING.pack(
+        kind, 0, r, v, *_rows("logits", logits, (r, v), logits.dtype, at), _array("uniform", uniform, one, _F32, at), _array("temperature", temperature, one, _F32, at),
+        _array("top_k", top_k, one, _I32, at), _array("top_p", top_p, one, _F32, at), _array("min_p", min_p, one, _F32, at),
+        _array("tokens", tokens, one, _I32, at), _array("chances", chances, one, _F32, at)))
     return tokens, chances

@@ -40,6 +40,9 @@ def scan(**kw):
 def test_struct_layouts_match_header():
     assert C.sizeof(capi.Convolution) == 4 * 4 + 3 * 8 + 4 * 24 + 9 * 8
     assert C.sizeof(capi.Scan) == 4 * 4 + 5 * 8 + 12 * 24 + 7 * 8 + 5 * 8
+    for s, packed in ((capi.Convolution, sequence._CONVOLUTION), (capi.Scan, sequence._SCAN), (capi.Distillation, sequence._DISTILLATION),
+                      (capi.Sampling, sequence._SAMPLING)):
+        assert C.sizeof(s) == packed.size
 
 
 @pytest.mark.parametrize("change,word", [(dict(type=3), "type"), (dict(taps=0), "taps"), (dict(taps=9), "taps"), (dict(time=1 << 31), "dimension"),
