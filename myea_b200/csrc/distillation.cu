@@ -3,11 +3,16 @@
 //   q_i = e^(c (x_i - m)) / s,  r_i = e^(x_i - m) / s1,   soft term = soft T^2 sum_k p_k (log p_k - c (x_k - m) + log s)
 //   gradient = soft T (q_i - sum of the p of word i) + hard (r_i - [i = label])
 //
-// Bound by memory: the row is read once from memory for m, s and s1 (in one pass: a sum is scaled whenever its maximum rises)
-// and a second time, out of L2, when the gradient is written.  A block, or a cluster of blocks where the rows alone leave SMs
-// idle, takes a row; the cluster's parts of the sums are exchanged through shared memory and joined in rank order.  The
-// teacher's few words are mended at the end: their gradients are formed again from the logits with the teacher's part, so every
-// element is rounded once.
+// Bound by memory, and nearly as much by the exponentials (two per word, 16 a cycle and SM).  Rows of up to 4096 packs of 16 bytes
+// stay in registers from the one time that they are read until their gradient is written.  Longer ones are read twice, the second
+// time out of L2: 296 rows of 256 KB at a time fit there as long as the gradients, which nobody reads here, are stored past it
+// (stored the ordinary way a third of the second reading came out of memory again).  2048 rows of 131072 bf16 logits: 252 us, 4.3 TB/s
+// of 6.5; a block of 1024 threads per SM 272 us, registers of clusters of four 422 us, most of it waiting for one another.
+// A cluster of blocks takes a row only where the rows leave SMs idle; the blocks' parts of the sums are exchanged through
+// shared memory and joined in rank order.
+// Exponents are formed from x - m, which is exact near the maximum, where it counts.  The first warp
+// works on the teacher's few words meanwhile; they are mended at the end: their gradients are formed again from the logits with the
+// teacher's part, so every element is rounded once.
 #include <cooperative_groups.h>
 
 #include "sequence.cuh"
@@ -16,174 +21,214 @@ namespace myea {
 namespace {
 
 namespace cg = cooperative_groups;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTopMost = 1024;
 
 template <typename T> struct Pack { static constexpr int N = 16 / sizeof(T); uint4 v; };
-template <typename T> __device__ __forceinline__ void unpack(const Pack<T> &p, float (&x)[Pack<T>::N]) {
-  const T *e = reinterpret_cast<const T *>(&p.v);
-#pragma unroll
-  for (int i = 0; i < Pack<T>::N; ++i) x[i] = to_float(e[i]);
+// the k-th pair of a pack's words
+__device__ __forceinline__ float2 pair(const Pack<float> &p, int k) {
+  return k == 0 ? make_float2(__uint_as_float(p.v.x), __uint_as_float(p.v.y)) : make_float2(__uint_as_float(p.v.z), __uint_as_float(p.v.w));
 }
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ uint32_t word(const uint4 &v, int k) { return k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w; }
+__device__ __forceinline__ float2 pair(const Pack<__nv_bfloat16> &p, int k) {
+  const uint32_t w = word(p.v, k);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 pair(const Pack<__half> &p, int k) {
+  const uint32_t w = word(p.v, k);
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t packed(float2 x, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t packed(float2 x, __half) {
+  const __half2 h = __floats2half2_rn(x.x, x.y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// the largest of a pack's words, NaN passed over
+template <typename T> __device__ __forceinline__ float largest(const Pack<T> &p) {
+  float2 m = pair(p, 0);
+#pragma unroll
+  for (int k = 1; k < Pack<T>::N / 2; ++k) {
+    const float2 x = pair(p, k);
+    m = make_float2(fmaxf(m.x, x.x), fmaxf(m.y, x.y));
+  }
+  return fmaxf(m.x, m.y);
 }
 
 // Maximum and sums of exponentials of what has been seen
 struct Running {
   float m = -INFINITY, s = 0.f, s1 = 0.f;   // s at the temperature, s1 at 1 (only where both are asked for)
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
   __device__ __forceinline__ void rise(float to, float c, bool two) {   // to >= m
-    const float by = to == -INFINITY ? 0.f : m - to;
+    if (to == m) return;
+    const float by = m == -INFINITY ? 0.f : m - to;   // (nothing has been summed yet)
     s *= exp2_fast(by * c);
     if (two) s1 *= exp2_fast(by * kLog2e);
     m = to;
   }
-  __device__ __forceinline__ void join(const Running &o, float c, bool two) {
-    Running r = o;
-    const float to = fmaxf(m, r.m);
+  // the lanes of a warp, every lane ending with the same
+  __device__ __forceinline__ void join_lanes(float c, bool two) {
+    float to = m;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, k));
     rise(to, c, two);
-    r.rise(to, c, two);
-    s += r.s;
-    s1 += r.s1;
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, k);
+      if (two) s1 += __shfl_xor_sync(0xffffffffu, s1, k);
+    }
   }
 };
 
-template <typename T, bool TWO>
-__global__ void __launch_bounds__(512) distillation_kernel(const myea_distillation d) {
+// P: packs of a thread at a time
+template <typename T, bool TWO, int P>
+__global__ void __launch_bounds__(512, 2) distillation_kernel(const myea_distillation d) {
   constexpr int E = Pack<T>::N;
   extern __shared__ float dynamic[];
   int *s_index = reinterpret_cast<int *>(dynamic);
   float *s_p = dynamic + d.top, *s_x = s_p + d.top;   // the teacher's probabilities, the logits of its words
-  __shared__ Running s_warp[16], s_part;
-  __shared__ float s_sum[17];
+  __shared__ Running s_warp[32], s_part;
+  __shared__ bool s_taught;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
   const long long row = blockIdx.x / parts;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-  const long long V = static_cast<long long>(d.vocabulary);
-  const int K = static_cast<int>(d.top);
+  const int V = static_cast<int>(d.vocabulary), K = static_cast<int>(d.top);
   const T *x = static_cast<const T *>(d.logits) + row * d.logits_stride;
   T *out = d.d_logits == nullptr ? nullptr : static_cast<T *>(d.d_logits) + row * d.d_logits_stride;
   // the row from its first 16-byte boundary on in packs, the blocks' shares of them, the elements before and behind
-  long long head = static_cast<long long>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T));
-  head = head < V ? head : V;
-  const long long packs = (V - head) / E, first = packs * part / parts, last = packs * (part + 1) / parts;
-  const long long from = part == 0 ? 0 : head + first * E, to = part == parts - 1 ? V : head + last * E;   // this block's elements
+  const int head = min(V, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+  const int packs = (V - head) / E, first = static_cast<int>(static_cast<long long>(packs) * part / parts);
+  const int last = static_cast<int>(static_cast<long long>(packs) * (part + 1) / parts);
+  const int from = part == 0 ? 0 : head + first * E, to = part == parts - 1 ? V : head + last * E;   // this block's elements
   const Pack<T> *body = reinterpret_cast<const Pack<T> *>(x + head);
   const bool out_packs = out != nullptr && aligned_16(out + head);
-  const float w = d.weight == nullptr ? 1.f : d.weight[row];
-  if (w == 0.f) {   // (every block of the row's cluster)
-    if (out != nullptr)
-      for (long long i = from + tid; i < to; i += threads) out[i] = from_float<T>(0.f);
-    if (part == 0 && tid == 0) d.losses[row] = 0.f;
-    return;
-  }
   const float c = kLog2e / d.temperature;
-
-  // the teacher's words and their logits
-  float t_max = -INFINITY;
-  for (int k = tid; k < K; k += threads) {
-    const int i = d.index[row * d.index_stride + k];
-    const bool there = i >= 0 && i < V;
-    const float t = there ? d.teacher[row * d.teacher_stride + k] : -INFINITY;
-    s_index[k] = there ? i : -1;
-    s_p[k] = t;
-    s_x[k] = there ? to_float(x[i]) : 0.f;
-    t_max = fmaxf(t_max, t);
-  }
+  Pack<T> p[P];
+  const int reach = P * threads;
+  const auto load = [&](int at) {
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+      if (at + u * threads < last) p[u] = body[at + u * threads];
+  };
+  load(first + tid);   // (under way while the row's weight is)
+  const float w = d.weight == nullptr ? 1.f : d.weight[row];
+  const auto nothing = [&]() {
+    if (out != nullptr)
+      for (int i = from + tid; i < to; i += threads) out[i] = from_float<T>(0.f);
+    if (part == 0 && tid == 0) d.losses[row] = 0.f;
+  };
+  if (w == 0.f) return nothing();   // (every block of the row's cluster)
+  // an element outside the packs, one per thread at most (part 0: in front, the last part: behind)
+  const int loose = part == 0 && tid < head ? tid : part == parts - 1 && head + packs * E + tid < V && tid < E ? head + packs * E + tid : -1;
+  const int loose2 = parts == 1 && part == 0 && tid < head && head + packs * E + tid < V ? head + packs * E + tid : -1;
+  const float x_loose = loose >= 0 ? to_float(x[loose]) : -INFINITY, x_loose2 = loose2 >= 0 ? to_float(x[loose2]) : -INFINITY;
   const int label = d.labels == nullptr || d.hard == 0.f ? -1 : d.labels[row];
   const bool labelled = label >= 0 && label < V;
   const float x_label = labelled ? to_float(x[label]) : 0.f;
-  t_max = block_max(t_max, s_sum);
-  float t_sum = 0.f;
-  for (int k = tid; k < K; k += threads) {
-    const float e = s_index[k] >= 0 && s_p[k] != -INFINITY ? exp2_fast((s_p[k] - t_max) * c) : 0.f;   // (NaN stays NaN)
-    s_p[k] = e;
-    t_sum += e;
-  }
-  t_sum = block_sum(t_sum, s_sum);
-  const bool taught = t_sum != 0.f;
-  const float t_scale = taught ? 1.f / t_sum : 0.f;
-  for (int k = tid; k < K; k += threads) s_p[k] *= t_scale;
 
-  // one pass for the maximum and the sums
+  if (warp == 0) {   // the teacher's words, their logits and probabilities
+    float t_max = -INFINITY;
+#pragma unroll 4
+    for (int k = lane; k < K; k += 32) {
+      const int i = d.index[row * d.index_stride + k];
+      const bool there = i >= 0 && i < V;
+      const float t = there ? d.teacher[row * d.teacher_stride + k] : -INFINITY;
+      s_index[k] = there ? i : -1;
+      s_p[k] = t;
+      s_x[k] = there ? to_float(x[i]) : 0.f;
+      t_max = fmaxf(t_max, t);
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) t_max = fmaxf(t_max, __shfl_xor_sync(0xffffffffu, t_max, m));
+    float t_sum = 0.f;
+    for (int k = lane; k < K; k += 32) {
+      const float e = s_index[k] >= 0 && s_p[k] != -INFINITY ? exp2_fast((s_p[k] - t_max) * c) : 0.f;   // (NaN stays NaN)
+      s_p[k] = e;
+      t_sum += e;
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) t_sum += __shfl_xor_sync(0xffffffffu, t_sum, m);
+    const float t_scale = t_sum != 0.f ? 1.f / t_sum : 0.f;
+    for (int k = lane; k < K; k += 32) s_p[k] *= t_scale;
+    if (lane == 0) s_taught = t_sum != 0.f;
+  }
+
+  // maximum and sums
   Running run;
-  const auto take = [&](const float *e, int n) {
-    float m = run.m;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, e[i]);
-    if (m > run.m) run.rise(m, c, TWO);
-    const float base = run.m == -INFINITY ? 0.f : run.m;
-    for (int i = 0; i < n; ++i) {
-      run.s += exp2_fast((e[i] - base) * c);
-      if (TWO) run.s1 += exp2_fast((e[i] - base) * kLog2e);
-    }
-  };
-  if (part == 0)
-    for (long long i = tid; i < head; i += threads) {
-      const float e[1] = {to_float(x[i])};
-      take(e, 1);
-    }
-  constexpr int U = 4;
-  for (long long i = first + tid; i < last; i += U * threads) {
-    Pack<T> p[U];
+  for (int at = first + tid;;) {
+    Pack<T> ahead[P];   // of a long row: the next packs are on their way while these are summed
+    if constexpr (P == 4) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * threads < last) p[u] = body[i + u * threads];
+      for (int u = 0; u < P; ++u)
+        if (at + reach + u * threads < last) ahead[u] = body[at + reach + u * threads];
+    }
+    float m = fmaxf(run.m, fmaxf(x_loose, x_loose2));
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * threads < last) {
-        float e[E];
-        unpack(p[u], e);
-        take(e, E);
+    for (int u = 0; u < P; ++u)
+      if (at + u * threads < last) m = fmaxf(m, largest(p[u]));
+    run.rise(m, c, TWO);
+    const float2 b = both(-run.base());
+    float2 s = both(0.f), s1 = both(0.f);
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+      if (at + u * threads < last) {
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          const float2 e = add2(pair(p[u], k), b);
+          s = add2(s, exp2_fast(mul2(e, both(c))));
+          if (TWO) s1 = add2(s1, exp2_fast(mul2(e, both(kLog2e))));
+        }
       }
-  }
-  if (part == parts - 1)
-    for (long long i = head + packs * E + tid; i < V; i += threads) {
-      const float e[1] = {to_float(x[i])};
-      take(e, 1);
-    }
-  // lanes, warps, blocks of the cluster: every block ends with the same sums
+    run.s += s.x + s.y;
+    run.s1 += s1.x + s1.y;
+    if (at - tid + reach >= last) break;
+    at += reach;
+    if constexpr (P == 4) {
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    Running o;
-    o.m = __shfl_xor_sync(0xffffffffu, run.m, m);
-    o.s = __shfl_xor_sync(0xffffffffu, run.s, m);
-    o.s1 = __shfl_xor_sync(0xffffffffu, run.s1, m);
-    run.join(o, c, TWO);
+      for (int u = 0; u < P; ++u) p[u] = ahead[u];
+    } else {
+      load(at);
+    }
   }
+  if (loose >= 0) {
+    run.s += exp2_fast((x_loose - run.base()) * c);
+    if (TWO) run.s1 += exp2_fast((x_loose - run.base()) * kLog2e);
+  }
+  if (loose2 >= 0) {
+    run.s += exp2_fast((x_loose2 - run.base()) * c);
+    if (TWO) run.s1 += exp2_fast((x_loose2 - run.base()) * kLog2e);
+  }
+  // lanes, warps, blocks of the cluster: every block ends with the same sums
+  run.join_lanes(c, TWO);
   if (lane == 0) s_warp[warp] = run;
   __syncthreads();
-  run = s_warp[0];
-  for (int k = 1; k < warps; ++k) run.join(s_warp[k], c, TWO);
+  run = lane < warps ? s_warp[lane] : Running();
+  run.join_lanes(c, TWO);
   if (parts > 1) {
     if (tid == 0) s_part = run;
     cluster.sync();
-    run = *cluster.map_shared_rank(&s_part, 0);
-    for (int k = 1; k < parts; ++k) run.join(*cluster.map_shared_rank(&s_part, k), c, TWO);
+    run = lane < parts ? *cluster.map_shared_rank(&s_part, lane) : Running();
+    run.join_lanes(c, TWO);
     cluster.sync();   // nobody leaves, or writes over the logits, while others read
   }
-  const float unit = TWO ? run.s1 : run.s;
-  if (run.s == 0.f) {   // no open word
-    if (out != nullptr)
-      for (long long i = from + tid; i < to; i += threads) out[i] = from_float<T>(0.f);
-    if (part == 0 && tid == 0) d.losses[row] = 0.f;
-    return;
-  }
+  if (run.s == 0.f) return nothing();   // no open word
+  const bool taught = s_taught;
+  const float top = run.m, unit = TWO ? run.s1 : run.s;
 
-  if (part == 0) {
+  if (part == 0 && warp == 0) {
     float kl = 0.f;
-    const float log_s = logf(run.s), T_ = d.temperature;
-    for (int k = tid; k < K; k += threads) {
-      const float p = s_p[k];
-      if (p != 0.f) kl += p * (logf(p) - (s_x[k] - run.m) / T_ + log_s);
+    const float log_s = logf(run.s);
+    for (int k = lane; k < K; k += 32) {
+      const float q = s_p[k];
+      if (q != 0.f) kl += q * (logf(q) - (s_x[k] - top) / d.temperature + log_s);
     }
-    kl = block_sum(kl, s_sum);
-    if (tid == 0) {
-      float loss = taught ? d.soft * T_ * T_ * kl : 0.f;
-      if (labelled) loss += d.hard * (logf(unit) - (x_label - run.m));
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, m);
+    if (lane == 0) {
+      float loss = taught ? d.soft * d.temperature * d.temperature * kl : 0.f;
+      if (labelled) loss += d.hard * (logf(unit) - (x_label - top));
       d.losses[row] = w * loss;
     }
   }
@@ -192,39 +237,39 @@ __global__ void __launch_bounds__(512) distillation_kernel(const myea_distillati
   // without a second temperature both terms have the same exponentials
   const float soft = taught ? w * d.soft * d.temperature : 0.f, hard = labelled ? w * d.hard : 0.f;
   const float a = TWO ? soft / run.s : (soft + hard) / run.s, b = TWO ? hard / run.s1 : 0.f;
-  const float base = run.m;
-  const auto gradient = [&](float e) {
-    float g = a * exp2_fast((e - base) * c);
-    if (TWO) g += b * exp2_fast((e - base) * kLog2e);
+  const auto gradient2 = [&](float2 e) {
+    const float2 far = add2(e, both(-top));
+    float2 g = mul2(both(a), exp2_fast(mul2(far, both(c))));
+    if (TWO) g = fma2(both(b), exp2_fast(mul2(far, both(kLog2e))), g);
     return g;
   };
-  if (part == 0)
-    for (long long i = tid; i < head; i += threads) out[i] = from_float<T>(gradient(to_float(x[i])));
-  for (long long i = first + tid; i < last; i += U * threads) {
-    Pack<T> p[U];
+  const auto gradient = [&](float e) { return gradient2(both(e)).x; };
+  const bool again = last - first > reach;
+  for (int at = first + tid; at - tid < last; at += reach) {
+    if (again) load(at);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * threads < last) p[u] = body[i + u * threads];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * threads < last) {
-        float e[E];
-        unpack(p[u], e);
+    for (int u = 0; u < P; ++u)
+      if (at + u * threads < last) {
         Pack<T> g;
-        T *ge = reinterpret_cast<T *>(&g.v);
-#pragma unroll
-        for (int k = 0; k < E; ++k) ge[k] = from_float<T>(gradient(e[k]));
-        T *at = out + head + (i + u * threads) * E;
-        if (out_packs) {
-          *reinterpret_cast<uint4 *>(at) = g.v;
+        if constexpr (E == 4) {
+          const float2 lo = gradient2(pair(p[u], 0)), hi = gradient2(pair(p[u], 1));
+          g.v = make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y));
         } else {
+          g.v = make_uint4(packed(gradient2(pair(p[u], 0)), T()), packed(gradient2(pair(p[u], 1)), T()), packed(gradient2(pair(p[u], 2)), T()),
+                           packed(gradient2(pair(p[u], 3)), T()));
+        }
+        T *to_ = out + head + static_cast<long long>(at + u * threads) * E;
+        if (out_packs) {
+          __stcs(reinterpret_cast<uint4 *>(to_), g.v);   // (nobody reads it here: what is read again stays in L2)
+        } else {
+          const T *ge = reinterpret_cast<const T *>(&g.v);
 #pragma unroll
-          for (int k = 0; k < E; ++k) at[k] = ge[k];
+          for (int k = 0; k < E; ++k) to_[k] = ge[k];
         }
       }
   }
-  if (part == parts - 1)
-    for (long long i = head + packs * E + tid; i < V; i += threads) out[i] = from_float<T>(gradient(to_float(x[i])));
+  if (loose >= 0) out[loose] = from_float<T>(gradient(x_loose));
+  if (loose2 >= 0) out[loose2] = from_float<T>(gradient(x_loose2));
   __syncthreads();
   // the teacher's words of this block's share, each by its first entry, and the label if the teacher does not name it
   bool named = false;
@@ -232,14 +277,14 @@ __global__ void __launch_bounds__(512) distillation_kernel(const myea_distillati
     const int i = s_index[k];
     if (i < from || i >= to) continue;
     bool leads = true;
-    float p = 0.f;
+    float q = 0.f;
     for (int j = 0; j < K; ++j) {
       if (s_index[j] != i) continue;
       if (j < k) leads = false;
-      p += s_p[j];
+      q += s_p[j];
     }
     if (i == label) named = true;
-    if (leads) out[i] = from_float<T>(gradient(s_x[k]) - soft * p - (i == label ? hard : 0.f));
+    if (leads) out[i] = from_float<T>(gradient(s_x[k]) - soft * q - (i == label ? hard : 0.f));
   }
   named = __syncthreads_or(named);
   if (tid == 0 && labelled && !named && label >= from && label < to) out[label] = from_float<T>(gradient(x_label) - hard);
@@ -257,11 +302,7 @@ const char *check(const myea_distillation *d) {
   return nullptr;
 }
 
-template <typename T> cudaError_t launch(const myea_distillation &d, cudaStream_t stream) {
-  int threads = 512, parts = 1;
-  while (threads > 128 && threads * (16 / sizeof(T)) * 2 > d.vocabulary) threads /= 2;
-  // a row over several blocks where the rows leave SMs idle, as long as a block keeps 8 packs per thread
-  while (parts < 8 && d.rows * parts * 2 <= 2ull * kSms && d.vocabulary / (parts * 2) >= threads * (16 / sizeof(T)) * 8) parts *= 2;
+template <typename T, int P> cudaError_t launch(const myea_distillation &d, int threads, int parts, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(d.rows * parts));
   cfg.blockDim = dim3(threads);
@@ -273,7 +314,17 @@ template <typename T> cudaError_t launch(const myea_distillation &d, cudaStream_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const bool two = d.hard != 0.f && d.temperature != 1.f && d.labels != nullptr;
-  return two ? cudaLaunchKernelEx(&cfg, distillation_kernel<T, true>, d) : cudaLaunchKernelEx(&cfg, distillation_kernel<T, false>, d);
+  return two ? cudaLaunchKernelEx(&cfg, distillation_kernel<T, true, P>, d) : cudaLaunchKernelEx(&cfg, distillation_kernel<T, false, P>, d);
+}
+
+template <typename T> cudaError_t launch(const myea_distillation &d, cudaStream_t stream) {
+  const uint64_t packs = (d.vocabulary * sizeof(T) + 15) / 16;
+  int parts = 1;
+  while (parts < 8 && d.rows * parts * 2 <= 2ull * kSms && packs >= parts * 2 * 256) parts *= 2;
+  const uint64_t share = (packs + parts - 1) / parts;
+  if (share <= 1024) return launch<T, 2>(d, share <= 64 ? 32 : static_cast<int>((share / 2 + 31) / 32 * 32), parts, stream);
+  if (share <= 4096) return launch<T, 8>(d, 512, parts, stream);
+  return launch<T, 4>(d, 512, parts, stream);
 }
 
 }  // namespace

@@ -24,7 +24,7 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kParts = 8, kList = 1024;
 static_assert(kThreads == 256, "a thread makes one entry of the table");
-constexpr double kLog2e = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
+constexpr double kLog2e64 = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
 template <typename T> struct Pack { static constexpr int N = 16 / sizeof(T); uint4 v; };
 
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
   d.m = m;
   d.md = static_cast<double>(m);
   d.half_scale = 2.f / temperature;
-  d.per = 256.0 * kLog2e / static_cast<double>(temperature);
+  d.per = 256.0 * kLog2e64 / static_cast<double>(temperature);
   d.shift = shift;
   d.beyond = static_cast<float>((shift + 1) * kLn2) + 0.5f;
 

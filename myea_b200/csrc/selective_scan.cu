@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(2 * S::NT) scan_forward_kernel(const ScanArgs 
 // where many sequences are answered at once.  The arithmetic is that of the kernel above, in its order: tokens one by one give
 // the bits of the whole sequence.
 template <typename T, int LPC>
-__global__ void __launch_bounds__(256) scan_steps_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(256, 4) scan_steps_kernel(const ScanArgs a) {
   const unsigned id = blockIdx.x * blockDim.x + threadIdx.x;
   const unsigned pairs = (a.per_group + 1) / 2, pair_id = id / LPC;
   const int l = static_cast<int>(id % LPC), n = l * 4;
@@ -166,16 +166,24 @@ __global__ void __launch_bounds__(256) scan_steps_kernel(const ScanArgs a) {
   const auto two = [&](const float *p) { return p == nullptr ? both(0.f) : make_float2(channels > 0 ? p[c] : 0.f, channels > 1 ? p[c + 1] : 0.f); };
   bias = two(a.s.delta_bias);
   skip = two(a.s.D);
+  float4 ahead[2];   // the next sequence's states are on their way while this one's step is made
+  const auto load = [&](long long b) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      ahead[q] = a.s.state != nullptr && b < a.batch
+                     ? load_states(a.s.state + (b * a.width + c + q) * a.states + n, q < channels ? min(4, a.states - n) : 0, a.vec_state)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(blockIdx.y);
   for (int sequence = blockIdx.y; sequence < a.batch; sequence += gridDim.y) {
     const long long b = sequence;
     const int length = sequence_length(a.s.lengths, b, a.time);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int have = q < channels ? min(4, a.states - n) : 0;
-      const float4 start = a.s.state != nullptr ? load_states(a.s.state + (b * a.width + c + q) * a.states + n, have, a.vec_state) : make_float4(0.f, 0.f, 0.f, 0.f);
-      h[q][0] = lo(start);
-      h[q][1] = hi(start);
+      h[q][0] = lo(ahead[q]);
+      h[q][1] = hi(ahead[q]);
     }
+    load(b + gridDim.y);
     if (a.s.checkpoints != nullptr) {
 #pragma unroll
       for (int q = 0; q < 2; ++q)

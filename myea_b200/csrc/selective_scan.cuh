@@ -25,7 +25,7 @@ namespace myea {
 namespace scan {
 
 constexpr int TT = 16;   // positions of a tile, and between checkpoints
-constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.925963033500e-8f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2eRest = 1.925963033500e-8f, kLn2 = 0.6931471805599453f;
 
 struct ScanArgs {
   myea_scan s;
@@ -82,19 +82,7 @@ template <int LPC_, int CPT_> struct Shape {
   static constexpr int BC = TT * NP;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
-__device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
-__device__ __forceinline__ float2 exp2_fast(float2 x) { return make_float2(exp2_fast(x.x), exp2_fast(x.y)); }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float min_nan(float a, float b) {   // (NaN stays)
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -105,13 +93,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float inverse(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float2 inverse2(float2 x) { return make_float2(inverse(x.x), inverse(x.y)); }
-
 // log(1 + e^x) of two values, and its slope.  With e = e^-|x| <= 1 and q = e / (2 + e) <= 1/3:  log(1 + e) = 2 atanh(q) = 2 (q + q^3 / 3 +
 // ...), whose first term left out, q^15 / 15, is below 2^-26 of the sum.  The product |x| log2(e) is carried to 48 bits.
 template <bool SLOPE> __device__ __forceinline__ float2 softplus2(float2 x, float2 &slope) {
@@ -142,11 +123,6 @@ __device__ __forceinline__ float4 step_lengths(float4 raw, float4 bias, bool sof
     s1 = softplus2<false>(s1, slope);
   }
   return there ? make_float4(s0.x, s0.y, s1.x, s1.y) : make_float4(0.f, 0.f, 0.f, 0.f);
-}
-// z * sigmoid(z), and sigmoid(z)
-__device__ __forceinline__ float2 gate2(float2 z, float2 &sig) {
-  sig = inverse2(add2(exp2_fast(mul2(z, both(-kLog2e))), both(1.f)));
-  return mul2(z, sig);
 }
 __device__ __forceinline__ float4 gated(float4 y, float4 z) {
   float2 sig;

@@ -14,6 +14,7 @@ namespace myea {
 
 constexpr uint64_t kSequenceMost = uint64_t(1) << 30;   // of any one dimension
 constexpr int kSms = 148;
+constexpr float kLog2e = 1.4426950408889634f;
 
 inline int refuse(char *dst, size_t cap, int code, const char *msg) {
   if (dst != nullptr && cap > 0) snprintf(dst, cap, "%s", msg);
@@ -124,35 +125,37 @@ __device__ __forceinline__ float4 parameters4(const float *p, int n, float none 
   }
   return r;
 }
-// (a denominator beyond 2^126 divides to 0, which is the limit)
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// 2^x and 1 / x to two steps, denormals as 0
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two values in one instruction
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 lo(float4 v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi(float4 v) { return make_float2(v.z, v.w); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 exp2_fast(float2 x) { return make_float2(exp2_fast(x.x), exp2_fast(x.y)); }
+__device__ __forceinline__ float2 inverse2(float2 x) { return make_float2(inverse(x.x), inverse(x.y)); }
+// z * sigmoid(z), and sigmoid(z)  (beyond the range of e^-z it is 0, the limit)
+__device__ __forceinline__ float2 gate2(float2 z, float2 &sig) {
+  sig = inverse2(add2(exp2_fast(mul2(z, both(-kLog2e))), both(1.f)));
+  return mul2(z, sig);
+}
+__device__ __forceinline__ float sigmoid(float x) { return inverse(1.f + exp2_fast(x * -kLog2e)); }
 __device__ __forceinline__ int sequence_length(const int32_t *lengths, long long b, int time) {
   return lengths == nullptr ? time : min(max(lengths[b], 0), time);
 }
 
 __device__ __forceinline__ bool aligned_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// over all threads of a block of at most 512, in a fixed order; memory: 17 floats that nothing else uses meanwhile
-__device__ __forceinline__ float block_sum(float x, float *memory) {
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) memory[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = 0.f;
-  for (int k = 0; k < static_cast<int>(blockDim.x >> 5); ++k) x += memory[k];
-  return x;
-}
-__device__ __forceinline__ float block_max(float x, float *memory) {
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) memory[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = memory[0];
-  for (int k = 1; k < static_cast<int>(blockDim.x >> 5); ++k) x = fmaxf(x, memory[k]);
-  return x;
-}
-
 // store(column, sum over rows of part[row][column]): partial sums of blocks that ran side by side, 32 columns and 8 strands of
 // rows per block of 256 threads, the strands joined in their order
 template <typename Store>
