@@ -40,6 +40,10 @@ extern "C" {
 #define MYEA_LAYER_LSTM 8u
 #define MYEA_LAYER_MAX_POOLING 9u     /* the same five values */
 #define MYEA_LAYER_RESIDUAL 10u
+#define MYEA_LAYER_SELECTIVE_SCAN 100u /* no counterpart in the reference: a short causal convolution and a selective state space scan over the
+   time steps (myea_scan below).  unit_parameters: units D, states N (1 to 128), taps (1 to 8).  Reads a hidden fully connected
+   layer of 3 D + 2 N neurons that projects to [x (D) | gate (D) | step (D) | B (N) | C (N)]; its parameters are one run of the weights:
+   [convolution D x taps | its bias D | rates a, D x N, A = -e^a | skip D | step bias D].  No dropout, no normalization, not in checkpoint files. */
 /* ENUM_TYPE_NETWORKS (Enum_Type_Networks.hpp:25) */
 #define MYEA_NETWORK_AUTOENCODER 1u
 #define MYEA_NETWORK_FEEDFORWARD 3u
@@ -310,6 +314,17 @@ int myea_b200_forward_device(myea_handle h, uint64_t batch, const float *device_
  * ptr_array_number_loss, ptr_array_accuracy_values) and read with myea_b200_get_loss. */
 int myea_b200_compute_error(myea_handle h, uint64_t batch, const float *desired_TBO);
 int myea_b200_compute_error_device(myea_handle h, uint64_t batch, const float *device_desired_TBO);
+/* No counterpart in the reference.  Instead of compute_error, for a softmax output layer and the cross entropy: the error against a
+ * teacher's best logits (myea_distillation below) for the rows that compute_error would score, [T][batch] lists of `top` entries in DEVICE
+ * memory on this handle's GPU: index and teacher [T][batch][top], labels and weight [T][batch] (may be null).  Losses are
+ * ACCUMULATED as by compute_error, `outputs` terms per row; accuracy is not scored.  Asynchronous on the handle's stream. */
+int myea_b200_compute_error_distillation_device(myea_handle h, uint64_t batch, const int32_t *index, const float *teacher, uint64_t top,
+                                                const int32_t *labels, const float *weight, float temperature, float soft, float hard);
+/* No counterpart in the reference.  Draws one output of a softmax output layer for every row of the last forward pass (myea_sampling below),
+ * [T][batch] values per array in DEVICE memory on this handle's GPU; settings and chances may be null.  Asynchronous on the
+ * handle's stream. */
+int myea_b200_sample_outputs_device(myea_handle h, uint64_t batch, const float *uniform, const float *temperature, const int32_t *top_k,
+                                    const float *top_p, const float *min_p, int32_t *tokens, float *chances);
 /* Reset__Loss (Data.hpp:823) / the accumulators behind Get__Loss (Data.hpp:2913). */
 int myea_b200_reset_loss(myea_handle h);
 int myea_b200_get_loss(myea_handle h, double *loss_sum, uint64_t *number_loss, double *accuracy_sum);

@@ -16,6 +16,7 @@ NET_AUTOENCODER = 1
 LAYER_FC, LAYER_LSTM, LAYER_RESIDUAL = 4, 8, 10
 LAYER_AVERAGE_POOLING, LAYER_MAX_POOLING = 1, 9
 LAYER_FC_IND_RNN = 5
+LAYER_SELECTIVE_SCAN = 100
 NET_FEEDFORWARD, NET_RECURRENT = 3, 4
 AF_ELU, AF_LINEAR, AF_LEAKY_RELU, AF_RELU, AF_SELU, AF_SIGMOID, AF_SOFTMAX, AF_TANH = 3, 11, 14, 16, 17, 18, 22, 23
 (AF_COSINE, AF_COSINE_SYMMETRIC, AF_ELLIOT, AF_ELLIOT_SYMMETRIC, AF_GAUSSIAN, AF_GAUSSIAN_STEPWISE, AF_GAUSSIAN_SYMMETRIC, AF_ISRU, AF_ISRLU,
@@ -136,6 +137,19 @@ def pooling(kind, kernel, stride, padding=0, dilation=1, ceil_mode=False):
     return d
 
 
+def selective_scan(units, states=16, taps=4):
+    """causal convolution and selective state space scan; reads a fully connected layer of selective_scan_inputs(units, states) neurons"""
+    d = LayerDesc()
+    d.type_layer = LAYER_SELECTIVE_SCAN
+    d.unit_parameters[0], d.unit_parameters[1], d.unit_parameters[2] = units, states, taps
+    return d
+
+
+def selective_scan_inputs(units, states=16):
+    """neurons of the layer below a selective scan layer: [x | gate | step | B | C]"""
+    return 3 * units + 2 * states
+
+
 def lstm(blocks, cells_per_block=1, bidirectional=False, dropout=DROP_NONE, p=(0.0, 0.0, 0.0)):
     d = LayerDesc()
     d.type_layer = LAYER_LSTM
@@ -167,7 +181,7 @@ def net(layers, batch, T=1, loss=LOSS_MSE, accuracy=ACC_NONE, time_delays=0, mom
     (0.999, 1e-5, 1, 0: Data.hpp:2966-2969)."""
     d = NetDesc()
     d.number_layers = len(layers)
-    d.type_network = NET_RECURRENT if T > 1 or any(l.type_layer in (LAYER_LSTM, LAYER_FC_IND_RNN) for l in layers) else NET_FEEDFORWARD
+    d.type_network = NET_RECURRENT if T > 1 or any(l.type_layer in (LAYER_LSTM, LAYER_FC_IND_RNN, LAYER_SELECTIVE_SCAN) for l in layers) else NET_FEEDFORWARD
     d.number_recurrent_depth = T
     d.number_time_delays = time_delays
     d.batch_size = batch
@@ -240,6 +254,9 @@ _PROTOS = {
     "myea_b200_forward_device": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_int]),
     "myea_b200_compute_error": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p]),
     "myea_b200_compute_error_device": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p]),
+    "myea_b200_compute_error_distillation_device": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_float,
+                                                              C.c_float, C.c_float]),
+    "myea_b200_sample_outputs_device": (C.c_int, [C.c_void_p, C.c_uint64] + [C.c_void_p] * 7),
     "myea_b200_reset_loss": (C.c_int, [C.c_void_p]),
     "myea_b200_get_loss": (C.c_int, [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_uint64), C.POINTER(C.c_double)]),
     "myea_b200_backward": (C.c_int, [C.c_void_p, C.c_uint64]),

@@ -129,7 +129,13 @@ int myea::build_index_map(myea_b200_net *net) {
           return fail(net, MYEA_E_INVALID, "pooling layers take neither dropout nor normalization");
         L.n_out = pooling_output_width(d.layers[l], net->layers[l - 1].n_out);
         break;
-      default: return fail(net, MYEA_E_UNSUPPORTED, "layer type not built (fully connected, LSTM, residual, average / max pooling)");
+      case MYEA_LAYER_SELECTIVE_SCAN:
+        // its parameters go by the width of the layer that it reads, which propagates the error of its inputs
+        if (l < 2 || net->layers[l - 1].type != MYEA_LAYER_FULLY_CONNECTED)
+          return fail(net, MYEA_E_UNSUPPORTED, "a selective scan layer reads a hidden fully connected layer");
+        L.n_out = static_cast<long long>(d.layers[l].unit_parameters[0]);
+        break;
+      default: return fail(net, MYEA_E_UNSUPPORTED, "layer type not built (fully connected, LSTM, residual, average / max pooling, selective scan)");
     }
     if (L.type != MYEA_LAYER_RESIDUAL && L.n_out <= 0) return fail(net, MYEA_E_INVALID, "layer with zero units");
   }
@@ -155,6 +161,12 @@ int myea::build_index_map(myea_b200_net *net) {
     const uint32_t t = net->layers[l].type;
     if ((t == MYEA_LAYER_AVERAGE_POOLING || t == MYEA_LAYER_MAX_POOLING) && layer_in_block(net, static_cast<int>(l) - 1, nullptr))
       return fail(net, MYEA_E_UNSUPPORTED, "a pooling layer next to a residual block is not built");
+    if (t == MYEA_LAYER_SELECTIVE_SCAN) {
+      if (layer_in_block(net, static_cast<int>(l) - 1, nullptr) || layer_in_block(net, static_cast<int>(l), nullptr) || net->layers[l + 1].type == MYEA_LAYER_RESIDUAL)
+        return fail(net, MYEA_E_UNSUPPORTED, "a selective scan layer next to a residual block is not built");
+      const char *msg = nullptr;
+      if (scan_layer_parameters(net->layers[l].desc, net->layers[l - 1].n_out, &msg) == 0) return fail(net, MYEA_E_INVALID, msg);
+    }
   }
   // inputs: a layer reads the layer before it; the first layer of a residual block reads the layer before the
   // residual layer, and the layer after a block reads the block's output (held by the residual layer)
@@ -174,7 +186,7 @@ int myea::build_index_map(myea_b200_net *net) {
   uint64_t tw = 0;
   for (uint32_t l = 1; l < n; ++l) {
     LayerPlan &L = net->layers[l];
-    const bool has_connections = L.type == MYEA_LAYER_FULLY_CONNECTED || L.type == MYEA_LAYER_LSTM;
+    const bool has_connections = L.type == MYEA_LAYER_FULLY_CONNECTED || L.type == MYEA_LAYER_LSTM || L.type == MYEA_LAYER_SELECTIVE_SCAN;
     L.idx.number_inputs = has_connections ? L.n_in : 0;  // residual and pooling layers have no connections of their own
     L.idx.number_outputs = L.n_out;
     if (L.type == MYEA_LAYER_FULLY_CONNECTED) {
@@ -191,6 +203,11 @@ int myea::build_index_map(myea_b200_net *net) {
       L.idx.block_stride = cpb * (L.n_in + cells_dir) + 3 * L.n_in + 3 * cells_dir + 3 * cpb;
       L.idx.first_connection_index = tw;
       tw += blocks * L.idx.block_stride;
+      L.idx.last_connection_index = tw;
+    } else if (L.type == MYEA_LAYER_SELECTIVE_SCAN) {
+      const char *msg = nullptr;
+      L.idx.first_connection_index = tw;
+      tw += static_cast<uint64_t>(scan_layer_parameters(L.desc, L.n_in, &msg));
       L.idx.last_connection_index = tw;
     }
   }
@@ -236,7 +253,7 @@ int myea::build_index_map(myea_b200_net *net) {
         own = 3 * L.n_out + 6 * static_cast<long long>(d.layers[l].unit_parameters[0]) * dirs;
       }
       if (L.type == MYEA_LAYER_RESIDUAL) own = net->layers[l + L.block_depth].n_out;
-      if (L.type == MYEA_LAYER_AVERAGE_POOLING || L.type == MYEA_LAYER_MAX_POOLING) own = 0;  // Prepare__Normalized__Layer: none
+      if (L.type == MYEA_LAYER_AVERAGE_POOLING || L.type == MYEA_LAYER_MAX_POOLING || L.type == MYEA_LAYER_SELECTIVE_SCAN) own = 0;  // Prepare__Normalized__Layer: none
       else if (l > 0 && layer_in_block(net, static_cast<int>(l), nullptr)) own = L.n_in;
       L.idx.number_units_norm = static_cast<uint64_t>(own);
       units += static_cast<uint64_t>(own);
@@ -322,6 +339,11 @@ static int allocate_buffers(myea_b200_net *net) {
       RC(dev_alloc(net, &L.deriv, rows * L.n_out));
       L.errors = L.deriv;  // no activation of its own: the error on its outputs is the error its backward pass spreads
       if (L.type == MYEA_LAYER_MAX_POOLING) RC(dev_alloc(net, &L.pool_winner, rows * L.n_out));
+    } else if (L.type == MYEA_LAYER_SELECTIVE_SCAN) {
+      RC(dev_alloc(net, &L.values, rows * L.n_out));
+      RC(dev_alloc(net, &L.deriv, rows * L.n_out));
+      L.errors = L.deriv;  // the error on its outputs
+      RC(scan_layer_create(net, L));
     } else if (L.type == MYEA_LAYER_RESIDUAL) {
       RC(dev_alloc(net, &L.values, rows * L.n_out));
       RC(dev_alloc(net, &L.deriv, rows * L.n_out));
@@ -424,7 +446,7 @@ extern "C" void myea_b200_destroy(myea_handle net) {
   cudaSetDevice(net->ctx.device);
   if (net->ctx.stream) cudaStreamSynchronize(net->ctx.stream);
   comm_destroy(net);
-  for (auto &L : net->layers) lstm_destroy(L);
+  for (auto &L : net->layers) { lstm_destroy(L); scan_layer_destroy(L); }
   for (void *p : net->allocations) cudaFree(p);
   gemm_splitk_release(net->ctx);
   for (void *p : {static_cast<void *>(net->ds_inputs), static_cast<void *>(net->ds_outputs), static_cast<void *>(net->ds_order), static_cast<void *>(net->ds_loss)})
@@ -931,6 +953,9 @@ static int forward_impl(myea_b200_net *net, uint64_t batch, const float *src, cu
     } else if (L.type == MYEA_LAYER_AVERAGE_POOLING || L.type == MYEA_LAYER_MAX_POOLING) {
       RC(pooling_forward(net, L, in.values, rows));
       ++l;
+    } else if (L.type == MYEA_LAYER_SELECTIVE_SCAN) {
+      RC(scan_layer_forward(net, L));
+      ++l;
     } else {  // residual block: consumes layers l+1 .. l+depth
       RC(residual_forward(net, l));
       l += L.block_depth + 1;
@@ -1158,11 +1183,12 @@ extern "C" int myea_b200_backward(myea_handle net, uint64_t batch) {
     const int p = N.input_layer;
     if (p < 1) break;
     LayerPlan &P = net->layers[p];
-    const bool n_pool = N.type == MYEA_LAYER_AVERAGE_POOLING || N.type == MYEA_LAYER_MAX_POOLING;
+    const bool n_pool = N.type == MYEA_LAYER_AVERAGE_POOLING || N.type == MYEA_LAYER_MAX_POOLING, n_scan = N.type == MYEA_LAYER_SELECTIVE_SCAN;
     // the error of N carried to the outputs of P, without P's activation derivative
     auto send_plain = [&](float *dst) -> int {
       if (N.type == MYEA_LAYER_FULLY_CONNECTED) return fc_backward_from_fc(net, P, N, N.errors, rows, dst, false);
       if (n_pool) return pooling_backward(net, N, dst, rows);
+      if (n_scan) return scan_layer_backward(net, N, dst);
       return lstm_backward_to_input(net, N, dst, P, nullptr);
     };
     if (P.type == MYEA_LAYER_FULLY_CONNECTED) {
@@ -1210,9 +1236,9 @@ extern "C" int myea_b200_backward(myea_handle net, uint64_t batch) {
       }
       if (N.type == MYEA_LAYER_FULLY_CONNECTED) {
         RC(fc_backward_from_fc(net, P, N, N.errors, rows, P.deriv, true));
-      } else if (n_pool) {  // a pooling layer above: its backward pass has no epilogue to carry P's activation derivative
+      } else if (n_pool || n_scan) {  // a pooling or scan layer above: its backward pass has no epilogue to carry P's activation derivative
         P.bwd_fused_chunks = 0;
-        RC(pooling_backward(net, N, P.deriv, rows));
+        RC(send_plain(P.deriv));
         RC(activation_backward(net->ctx, P.deriv, P.summations, P.values, rows, P.n_out, P.desc.type_activation_function,
                                P.has_norm ? P.norm.col_scale : nullptr, P.has_norm ? P.norm.col_shift : nullptr));
       } else {  // an LSTM layer above: its input contraction carries P's activation derivative in the epilogue
@@ -1229,7 +1255,7 @@ extern "C" int myea_b200_backward(myea_handle net, uint64_t batch) {
     } else if (P.type == MYEA_LAYER_LSTM) {
       RC(send_plain(lstm_output_errors(P)));
       RC(lstm_backward(net, P));
-    } else if (P.type == MYEA_LAYER_AVERAGE_POOLING || P.type == MYEA_LAYER_MAX_POOLING) {
+    } else if (P.type == MYEA_LAYER_AVERAGE_POOLING || P.type == MYEA_LAYER_MAX_POOLING || P.type == MYEA_LAYER_SELECTIVE_SCAN) {
       RC(send_plain(P.deriv));  // P.errors == P.deriv: nothing of its own to finish
     } else {  // residual block feeding N: its output has no activation of its own
       if (N.type != MYEA_LAYER_FULLY_CONNECTED) return fail(net, MYEA_E_UNSUPPORTED, "a residual block below an LSTM or pooling layer is not built");
@@ -1323,6 +1349,8 @@ extern "C" int myea_b200_update_derivative_weight(myea_handle net, uint64_t batc
       }
     } else if (L.type == MYEA_LAYER_LSTM) {
       RC(lstm_update_derivative_weight(net, L, net->layers[L.input_layer].values, L.n_in));
+    } else if (L.type == MYEA_LAYER_SELECTIVE_SCAN) {
+      RC(scan_layer_update_derivative_weight(net, L));
     }
     if (net->comm != nullptr && L.idx.last_connection_index > L.idx.first_connection_index)
       RC(comm_reduce_bucket_async(net, L.idx.first_connection_index, L.idx.last_connection_index - L.idx.first_connection_index));

@@ -9,6 +9,7 @@
 namespace myea {
 
 struct LstmPlan;   // lstm.cu
+struct ScanLayer;  // net_sequence.cu
 struct LayerPlan;
 struct CommState;  // comm.cu
 
@@ -31,6 +32,7 @@ struct LayerPlan {
   float keep_scale = 1.f;             // factor applied to kept units while training
   float infer_scale = 1.f;            // factor applied to every unit at inference
   LstmPlan *lstm = nullptr;
+  ScanLayer *scan = nullptr;
   // residual block (type RESIDUAL): see residual.cu
   int block_depth = 0;
   uint8_t *shake_mask = nullptr;      // [B]
@@ -79,6 +81,14 @@ long long pooling_output_width(const myea_layer_desc &d, long long n_in);
 int pooling_forward(myea_b200_net *net, LayerPlan &L, const float *input, long long rows);
 int pooling_backward(myea_b200_net *net, LayerPlan &L, float *d_input, long long rows);
 
+// selective scan layers (net_sequence.cu)
+long long scan_layer_parameters(const myea_layer_desc &d, long long n_in, const char **msg);
+int scan_layer_create(myea_b200_net *net, LayerPlan &L);
+void scan_layer_destroy(LayerPlan &L);
+int scan_layer_forward(myea_b200_net *net, LayerPlan &L);
+int scan_layer_backward(myea_b200_net *net, LayerPlan &L, float *d_input);
+int scan_layer_update_derivative_weight(myea_b200_net *net, LayerPlan &L);
+
 // z = input * W^T of a fully connected layer and D = errors * W (error on the layer's inputs), from the layer's shared
 // operand panels when it has them, else through gemm_nt; `e` carries destination and fused extras (net.cu)
 // Where a kernel that produces the input of layer L (the array `input`), or the errors of layer L, leaves the operand panels
@@ -123,6 +133,7 @@ struct myea_b200_net {
   double *d_loss_acc = nullptr;  // [3] loss sum, accuracy sum, number of loss terms (an integer: d_loss_count)
   unsigned long long *d_loss_count = nullptr;
   double *d_sumsq = nullptr;
+  float *distillation_losses = nullptr;   // [T * B], made by the first error against a teacher
   float *d_clip_scale = nullptr;
   float optimizer_time_step = 0.f;
   float nosadam_previous_beta2 = 0.f;  // adam_previous_beta2 (Data.hpp:2953)

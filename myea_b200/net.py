@@ -162,6 +162,34 @@ class Net:
         Y = _f32(Y)
         self._ck(self.lib.myea_b200_compute_error(self.h, getattr(self, "active_B", self.B), Y.ctypes.data), "compute_error")
 
+    def _device_array(self, name, x, shape, dtype):
+        """address of an array on this network's GPU (a torch tensor); None where there is none"""
+        if x is None:
+            return None
+        if tuple(x.shape) != shape or not str(x.dtype).endswith(dtype) or not x.is_cuda or not x.is_contiguous():
+            raise ValueError("%s: expected a contiguous %s array %s on the GPU, got %s of %s on %s" % (name, dtype, shape, tuple(x.shape), x.dtype, x.device))
+        return x.data_ptr()
+
+    def compute_error_distillation(self, index, teacher, temperature=1.0, soft=1.0, hard=0.0, labels=None, weight=None):
+        """instead of compute_error: the error against a teacher's best logits, index (int32) and teacher (float32) [T, batch, top], labels (int32) and
+        weight (float32) [T, batch] on the GPU; what wrote them has to be done (the call runs on the network's stream)"""
+        rows = (self.T, getattr(self, "active_B", self.B))
+        top = int(index.shape[-1])
+        self._ck(self.lib.myea_b200_compute_error_distillation_device(
+            self.h, rows[1], self._device_array("index", index, rows + (top,), "int32"), self._device_array("teacher", teacher, rows + (top,), "float32"), top,
+            self._device_array("labels", labels, rows, "int32"), self._device_array("weight", weight, rows, "float32"), temperature, soft, hard),
+            "compute_error_distillation")
+
+    def sample_outputs(self, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, chances=None):
+        """draws one output for every row of the last forward pass into tokens (int32 [T, batch]), from uniform (float32 [T, batch] in [0, 1)) and
+        settings of that shape or None, all on the GPU; runs on the network's stream"""
+        rows = (self.T, getattr(self, "active_B", self.B))
+        at = self._device_array
+        self._ck(self.lib.myea_b200_sample_outputs_device(
+            self.h, rows[1], at("uniform", uniform, rows, "float32"), at("temperature", temperature, rows, "float32"), at("top_k", top_k, rows, "int32"),
+            at("top_p", top_p, rows, "float32"), at("min_p", min_p, rows, "float32"), at("tokens", tokens, rows, "int32"), at("chances", chances, rows, "float32")),
+            "sample_outputs")
+
     def backward(self):
         self._ck(self.lib.myea_b200_backward(self.h, getattr(self, "active_B", self.B)), "backward")
 
