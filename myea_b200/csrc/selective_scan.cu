@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(2 * S::NT) scan_forward_kernel(const ScanArgs 
           now = next;
         }
       }
-      __syncthreads();
+      meet();
     }
 #pragma unroll
     for (int q = 0; q < CPT; ++q) {
@@ -138,118 +138,126 @@ __global__ void __launch_bounds__(2 * S::NT) scan_forward_kernel(const ScanArgs 
           if (at < p.t1) y_rows.store(at - p.row, y);
         }
       }
-      __syncthreads();
+      meet();
     }
   }
 }
 
-// A few positions: nothing is staged, a thread loads what its two channels need where it lies.  Bound by the states' 8 bytes per value
-// where many sequences are answered at once.  The arithmetic is that of the kernel above, in its order: tokens one by one give
-// the bits of the whole sequence.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(256, 4) scan_steps_kernel(const ScanArgs a) {
-  const unsigned id = blockIdx.x * blockDim.x + threadIdx.x;
-  const unsigned pairs = (a.per_group + 1) / 2, pair_id = id / LPC;
-  const int l = static_cast<int>(id % LPC), n = l * 4;
-  const bool on = pair_id < pairs * a.groups;   // (threads beyond the last pair only take part in exchanges)
-  const int g = on ? static_cast<int>(pair_id / pairs) : 0, in_group = on ? static_cast<int>(pair_id % pairs) * 2 : 0;
-  const int c = g * a.per_group + in_group, channels = on ? min(2, a.per_group - in_group) : 0;
+// A few positions: bound by the states' 8 bytes per value where many sequences are answered at once.  A thread takes four states of one
+// channel in NB sequences, all of them under way at once; the step lengths, B and C come through shared memory, made once per channel
+// and sequence.  The sums are made in the order of the kernel above: tokens one by one give the bits of the whole sequence.
+template <typename T, int LPC, int NB>
+__global__ void __launch_bounds__(256, 3) scan_steps_kernel(const ScanArgs a, int tiles) {
+  constexpr int CH = 256 / LPC, NP = 4 * LPC, PAIRS = CH / 2 * NB, ITEMS = (PAIRS + 255) / 256;   // channels of a block; pairs of them in all sequences
+  __shared__ __align__(16) float2 s_step[NB * CH];   // step length, and times the input
+  __shared__ __align__(16) float s_y[NB * CH];
+  __shared__ __align__(16) float s_B[NB * NP], s_C[NB * NP];
+  const int tid = threadIdx.x, l = tid % LPC, n = l * 4, c = tid / LPC;
+  const int group = blockIdx.x / tiles, in_group = (blockIdx.x - group * tiles) * CH;
+  const int first = group * a.per_group + in_group, channels = min(CH, a.per_group - in_group);
+  const int have = c < channels ? min(4, a.states - n) : 0;
   const bool gate = a.s.z.data != nullptr;
-  float2 A[2][2], h[2][2], bias = both(0.f), skip = both(0.f);
+  const float4 a4 = load_states(a.s.A + static_cast<long long>(first + c) * a.states + n, have, a.vec_A);
+  const float2 A0 = make_float2(a4.x * kLog2e, a4.y * kLog2e), A1 = make_float2(a4.z * kLog2e, a4.w * kLog2e);
+  for (int b0 = blockIdx.y * NB; b0 < a.batch; b0 += gridDim.y * NB) {
+    float2 h[NB][2];
+    const long long held = static_cast<long long>(a.width) * a.states, own = static_cast<long long>(first + c) * a.states + n;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int have = q < channels ? min(4, a.states - n) : 0;
-    const float4 a4 = load_states(a.s.A + static_cast<long long>(c + q) * a.states + n, have, a.vec_A);
-    A[q][0] = make_float2(a4.x * kLog2e, a4.y * kLog2e);
-    A[q][1] = make_float2(a4.z * kLog2e, a4.w * kLog2e);
-  }
-  const auto two = [&](const float *p) { return p == nullptr ? both(0.f) : make_float2(channels > 0 ? p[c] : 0.f, channels > 1 ? p[c + 1] : 0.f); };
-  bias = two(a.s.delta_bias);
-  skip = two(a.s.D);
-  float4 ahead[2];   // the next sequence's states are on their way while this one's step is made
-  const auto load = [&](long long b) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      ahead[q] = a.s.state != nullptr && b < a.batch
-                     ? load_states(a.s.state + (b * a.width + c + q) * a.states + n, q < channels ? min(4, a.states - n) : 0, a.vec_state)
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
-  };
-  load(blockIdx.y);
-  for (int sequence = blockIdx.y; sequence < a.batch; sequence += gridDim.y) {
-    const long long b = sequence;
-    const int length = sequence_length(a.s.lengths, b, a.time);
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      h[q][0] = lo(ahead[q]);
-      h[q][1] = hi(ahead[q]);
+    for (int k = 0; k < NB; ++k) {
+      const float4 start = a.s.state != nullptr && b0 + k < a.batch ? load_states(a.s.state + (b0 + k) * held + own, have, a.vec_state) : make_float4(0.f, 0.f, 0.f, 0.f);
+      h[k][0] = lo(start);
+      h[k][1] = hi(start);
     }
-    load(b + gridDim.y);
-    if (a.s.checkpoints != nullptr) {
+    if (a.s.checkpoints != nullptr && c < channels && a.time > 0) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (q < channels && a.time > 0)
-          *reinterpret_cast<float4 *>(a.s.checkpoints + (b * a.width + c + q) * (4 * LPC) + n) = make_float4(h[q][0].x, h[q][0].y, h[q][1].x, h[q][1].y);
+      for (int k = 0; k < NB; ++k)
+        if (b0 + k < a.batch)
+          *reinterpret_cast<float4 *>(a.s.checkpoints + (static_cast<long long>(b0 + k) * a.width + first + c) * NP + n) = make_float4(h[k][0].x, h[k][0].y, h[k][1].x, h[k][1].y);
     }
-    const auto pair = [&](const myea_view &v, int t) {
-      const T *p = static_cast<const T *>(v.data) + b * v.stride_batch + t * v.stride_time + c;
-      return make_float2(channels > 0 ? to_float(p[0]) : 0.f, channels > 1 ? to_float(p[1]) : 0.f);
-    };
-    const auto four = [&](const myea_view &v, bool vec, int t) {
-      return widen(load4(static_cast<const T *>(v.data) + b * v.stride_batch + t * v.stride_time + g * static_cast<long long>(a.states) + n, on ? min(4, a.states - n) : 0, vec));
-    };
     for (int t = 0; t < a.time; ++t) {
-      float2 s = both(0.f), x = both(0.f), slope;
-      float4 b4 = make_float4(0.f, 0.f, 0.f, 0.f), c4 = b4;
-      if (t < length) {
-        x = pair(a.s.u, t);
-        s = add2(pair(a.s.delta, t), bias);
-        b4 = four(a.s.B, a.vec_B, t);
-        c4 = four(a.s.C, a.vec_C, t);
+      float2 x[ITEMS], z[ITEMS];
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int item = tid + 256 * i, k = item / (CH / 2), c2 = item % (CH / 2) * 2;
+        const long long b = b0 + k;
+        if (item >= PAIRS) break;
+        const int count = b < a.batch && t < sequence_length(a.s.lengths, b, a.time) ? min(2, channels - c2) : 0;
+        const auto two = [&](const myea_view &v) {
+          const T *at = static_cast<const T *>(v.data) + b * v.stride_batch + t * v.stride_time + first + c2;
+          return make_float2(count > 0 ? to_float(at[0]) : 0.f, count > 1 ? to_float(at[1]) : 0.f);
+        };
+        x[i] = two(a.s.u);
+        float2 s = two(a.s.delta), slope;
+        z[i] = gate ? two(a.s.z) : both(0.f);
+        if (a.s.delta_bias != nullptr) s = add2(s, make_float2(count > 0 ? a.s.delta_bias[first + c2] : 0.f, count > 1 ? a.s.delta_bias[first + c2 + 1] : 0.f));
         if (a.s.softplus) s = softplus2<false>(s, slope);
+        if (count == 0) s = both(0.f);
+        const float2 in = mul2(s, x[i]);
+        *reinterpret_cast<float4 *>(s_step + k * CH + c2) = make_float4(s.x, in.x, s.y, in.y);
       }
-      const float2 in = mul2(s, x);
-      float y[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float2 sq = both(q == 0 ? s.x : s.y), iq = both(q == 0 ? in.x : in.y);
-        h[q][0] = fma2(exp2_fast(mul2(sq, A[q][0])), h[q][0], mul2(iq, lo(b4)));
-        h[q][1] = fma2(exp2_fast(mul2(sq, A[q][1])), h[q][1], mul2(iq, hi(b4)));
-        const float2 r = fma2(h[q][1], hi(c4), mul2(h[q][0], lo(c4)));
-        y[q] = r.x + r.y;
-#pragma unroll
-        for (int m = 4; m < LPC; m *= 2) y[q] += __shfl_xor_sync(0xffffffffu, y[q], m);
-#pragma unroll
-        for (int m = 1; m < (LPC < 4 ? LPC : 4); m *= 2) y[q] += __shfl_xor_sync(0xffffffffu, y[q], m);
+      for (int item = tid; item < 2 * NB * LPC; item += 256) {   // B, then C
+        const bool is_B = item < NB * LPC;
+        const int j = is_B ? item : item - NB * LPC, k = j / LPC, m = j % LPC * 4;
+        const long long b = b0 + k;
+        const myea_view &v = is_B ? a.s.B : a.s.C;
+        const int count = b < a.batch && t < sequence_length(a.s.lengths, b, a.time) ? min(4, a.states - m) : 0;
+        const T *at = static_cast<const T *>(v.data) + b * v.stride_batch + t * v.stride_time + group * static_cast<long long>(a.states) + m;
+        at4((is_B ? s_B : s_C) + j * 4) = widen(load4(at, count, is_B ? a.vec_B : a.vec_C));
       }
-      if (l == 0 && channels > 0) {
-        float2 out = fma2(skip, x, make_float2(y[0], y[1])), sig;
-        if (gate) out = mul2(out, gate2(t < length ? pair(a.s.z, t) : both(0.f), sig));
-        if (t >= length) out = both(0.f);
-        T *to = static_cast<T *>(a.s.y.data) + b * a.s.y.stride_batch + t * a.s.y.stride_time + c;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const float2 step = s_step[k * CH + c];
+        const float4 b4 = at4(s_B + k * NP + n), c4 = at4(s_C + k * NP + n);
+        h[k][0] = fma2(exp2_fast(mul2(both(step.x), A0)), h[k][0], mul2(both(step.y), lo(b4)));
+        h[k][1] = fma2(exp2_fast(mul2(both(step.x), A1)), h[k][1], mul2(both(step.y), hi(b4)));
+        const float2 r = fma2(h[k][1], hi(c4), mul2(h[k][0], lo(c4)));
+        float y = r.x + r.y;
+#pragma unroll
+        for (int m = 4; m < LPC; m *= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
+#pragma unroll
+        for (int m = 1; m < (LPC < 4 ? LPC : 4); m *= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
+        if (l == 0) s_y[k * CH + c] = y;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int item = tid + 256 * i, k = item / (CH / 2), c2 = item % (CH / 2) * 2;
+        const long long b = b0 + k;
+        if (item >= PAIRS || b >= a.batch || c2 >= channels) continue;
+        const float2 skip = a.s.D == nullptr ? both(0.f) : make_float2(a.s.D[first + c2], c2 + 1 < channels ? a.s.D[first + c2 + 1] : 0.f);
+        float2 out = fma2(skip, x[i], *reinterpret_cast<const float2 *>(s_y + k * CH + c2)), sig;
+        if (gate) out = mul2(out, gate2(z[i], sig));
+        if (t >= sequence_length(a.s.lengths, b, a.time)) out = both(0.f);
+        T *to = static_cast<T *>(a.s.y.data) + b * a.s.y.stride_batch + t * a.s.y.stride_time + first + c2;
         to[0] = from_float<T>(out.x);
-        if (channels > 1) to[1] = from_float<T>(out.y);
+        if (c2 + 1 < channels) to[1] = from_float<T>(out.y);
       }
     }
     if (a.s.final_state != nullptr) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (q < channels) store_states(a.s.final_state + (b * a.width + c + q) * a.states + n, h[q][0], h[q][1], min(4, a.states - n), a.vec_final);
+      for (int k = 0; k < NB; ++k)
+        if (b0 + k < a.batch) store_states(a.s.final_state + (b0 + k) * held + own, h[k][0], h[k][1], have, a.vec_final);
     }
+    __syncthreads();
   }
+}
+
+template <typename T, int LPC, int NB> void launch_steps(const ScanArgs &a, cudaStream_t stream) {
+  const int channels = 256 / LPC, tiles = (a.per_group + channels - 1) / channels, down = (a.batch + NB - 1) / NB;
+  scan_steps_kernel<T, LPC, NB><<<dim3(static_cast<unsigned>(tiles * a.groups), static_cast<unsigned>(down < 65535 ? down : 65535)), 256, 0, stream>>>(a, tiles);
 }
 
 template <typename S> constexpr size_t forward_smem() { return (4 * S::PAIRS + 4 * S::BC + 2 * S::SUMS) * sizeof(float); }
 
 template <typename T, typename S> cudaError_t launch_forward(const ScanArgs &a, cudaStream_t stream) {
   const long long blocks = static_cast<long long>(a.tiles) * a.groups * a.batch;
-  // Measured at 4096 channels of 16 states: 16 sequences of 2 positions 6.0 us against 16.3 staged, of 4 8.6, but one of 4 6.3 against
-  // 4.0; 256 sequences of 4 127 us against 219, of 8 229 against 221.
-  if (a.time <= (blocks > 4 * kSms ? 6 : 2)) {
-    const long long threads = static_cast<long long>(a.groups) * ((a.per_group + 1) / 2) * S::LPC;
-    const int block = threads < 256 ? static_cast<int>((threads + 31) / 32 * 32) : 256;
-    const long long across = (threads + block - 1) / block, most = (16ll * kSms + across - 1) / across;
-    const long long down = a.batch < most ? a.batch : most < 65535 ? most : 65535;
-    scan_steps_kernel<T, S::LPC><<<dim3(static_cast<unsigned>(across), static_cast<unsigned>(down)), block, 0, stream>>>(a);
+  // Measured at 4096 channels of 16 states in bf16: 256 sequences of 1 / 4 positions 40 / 89 us against 215 / 219 staged, 16 of them 5.2 /
+  // 11.5 against 16; with a sequence per block, which a single one needs, 3.0 us against 4.0, but two positions 4.8.
+  const bool many = blocks >= 4 * kSms;
+  if (a.time <= (many ? 4 : 1)) {
+    if (many) launch_steps<T, S::LPC, 8>(a, stream);
+    else launch_steps<T, S::LPC, 1>(a, stream);
     return cudaSuccess;
   }
   constexpr int smem = static_cast<int>(forward_smem<S>());
@@ -324,6 +332,7 @@ ScanArgs arguments(const myea_scan *s) {
   a.vec_B = even && view_takes_vectors(s->B, t); a.vec_C = even && view_takes_vectors(s->C, t);
   if (a.per_group % 4 != 0 && a.groups > 1)   // a group's first channel is on no boundary of four
     a.vec_u = a.vec_delta = a.vec_z = a.vec_y = a.vec_dy = a.vec_du = a.vec_ddelta = a.vec_dz = false;
+  a.vec_dB = even && view_takes_vectors(s->dB, t); a.vec_dC = even && view_takes_vectors(s->dC, t);
   a.vec_A = even && aligned(s->A, 16);
   a.vec_state = even && aligned(s->state, 16); a.vec_final = even && aligned(s->final_state, 16);
   a.vec_d_final = even && aligned(s->d_final_state, 16); a.vec_d_state = even && aligned(s->d_state, 16);

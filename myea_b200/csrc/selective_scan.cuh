@@ -32,7 +32,7 @@ struct ScanArgs {
   int batch, time, width, states, groups, per_group;
   int tiles;           // of channels in a group
   int chunk, chunks;   // positions of a chunk (a multiple of TT), chunks
-  bool vec_u, vec_delta, vec_z, vec_y, vec_dy, vec_du, vec_ddelta, vec_dz, vec_B, vec_C, vec_A, vec_state, vec_final, vec_d_final, vec_d_state;
+  bool vec_u, vec_delta, vec_z, vec_y, vec_dy, vec_du, vec_ddelta, vec_dz, vec_B, vec_C, vec_dB, vec_dC, vec_A, vec_state, vec_final, vec_d_final, vec_d_state;
   float *carry;        // [batch][chunks][width][NP]: states (errors on the states) of chunks from a zero start, then where they start
   float *steps;        // [batch][chunks][width]: sum of a chunk's step lengths
   float *part_bc;      // [tiles][batch][time][groups][LPC][dB, dC][4]
@@ -140,6 +140,9 @@ __device__ __forceinline__ void put_pairs(float *p, float4 v) {
   at4(p) = make_float4(v.x, v.x, v.y, v.y);
   at4(p + 4) = make_float4(v.z, v.z, v.w, v.w);
 }
+
+// all warps of a block whose halves run different code: each warp arrives from where it is
+__device__ __forceinline__ void meet() { asm volatile("barrier.sync 0;" ::: "memory"); }
 
 // Which channels and positions a block works on, and a thread in it
 template <typename S> struct Place {
