@@ -209,8 +209,8 @@ __global__ void __launch_bounds__(256, 3) scan_steps_kernel(const ScanArgs a, in
       for (int k = 0; k < NB; ++k) {
         const float2 step = s_step[k * CH + c];
         const float4 b4 = at4(s_B + k * NP + n), c4 = at4(s_C + k * NP + n);
-        h[k][0] = fma2(exp2_fast(mul2(both(step.x), A0)), h[k][0], mul2(both(step.y), lo(b4)));
-        h[k][1] = fma2(exp2_fast(mul2(both(step.x), A1)), h[k][1], mul2(both(step.y), hi(b4)));
+        h[k][0] = fma2(decay2(both(step.x), A0), h[k][0], mul2(both(step.y), lo(b4)));
+        h[k][1] = fma2(decay2(both(step.x), A1), h[k][1], mul2(both(step.y), hi(b4)));
         const float2 r = fma2(h[k][1], hi(c4), mul2(h[k][0], lo(c4)));
         float y = r.x + r.y;
 #pragma unroll

@@ -93,6 +93,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// 2^(s A).  The unit's results lie 2.0e-8 below 2^x on the average of x in -0.35 .. 0 (measured against 64 bits), the same way at every
+// step, which a state of long memory adds up: 2^-25 in the exponent takes that off.  (A step of length 0 still keeps the state.)
+__device__ __forceinline__ float2 decay2(float2 s, float2 A) { return exp2_fast(fma2(s, A, both(2.98023224e-8f))); }
+
 // log(1 + e^x) of two values, and its slope.  With e = e^-|x| <= 1 and q = e / (2 + e) <= 1/3:  log(1 + e) = 2 atanh(q) = 2 (q + q^3 / 3 +
 // ...), whose first term left out, q^15 / 15, is below 2^-26 of the sum.  The product |x| log2(e) is carried to 48 bits.
 template <bool SLOPE> __device__ __forceinline__ float2 softplus2(float2 x, float2 &slope) {
@@ -259,8 +263,8 @@ template <typename S> struct Steps {
 #pragma unroll
       for (int q = 0; q < S::CPT; ++q) {
         s[j][q] = pair[q].x;
-        decay[j][q][0] = exp2_fast(mul2(pair[q], A[q][0]));
-        decay[j][q][1] = exp2_fast(mul2(pair[q], A[q][1]));
+        decay[j][q][0] = decay2(pair[q], A[q][0]);
+        decay[j][q][1] = decay2(pair[q], A[q][1]);
       }
       get_pairs<S::CPT>(in + (k + j) * 2 * S::CH, x[j]);
       b[j] = at4(B + (k + j) * S::NP);

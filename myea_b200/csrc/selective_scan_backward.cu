@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(S::NT) scan_backward_states_kernel(const ScanA
       const float4 c4 = at4(s_C + k * S::NP + p.n);
 #pragma unroll
       for (int q = 0; q < CPT; ++q) {
-        g[q][0] = mul2(exp2_fast(mul2(both(s[q]), A[q][0])), fma2(both(e[q]), lo(c4), g[q][0]));
-        g[q][1] = mul2(exp2_fast(mul2(both(s[q]), A[q][1])), fma2(both(e[q]), hi(c4), g[q][1]));
+        g[q][0] = mul2(decay2(both(s[q]), A[q][0]), fma2(both(e[q]), lo(c4), g[q][0]));
+        g[q][1] = mul2(decay2(both(s[q]), A[q][1]), fma2(both(e[q]), hi(c4), g[q][1]));
         sum[q] += s[q];
       }
     }
@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(2 * S::NT, S::LPC <= 2 ? 1 : 2) scan_backward_
             const float4 b4 = at4(B + k * S::NP);
 #pragma unroll
             for (int q = 0; q < CPT; ++q) {
-              h[q][0] = fma2(exp2_fast(mul2(both(s[q]), A[q][0])), h[q][0], mul2(both(x[q]), lo(b4)));
-              h[q][1] = fma2(exp2_fast(mul2(both(s[q]), A[q][1])), h[q][1], mul2(both(x[q]), hi(b4)));
+              h[q][0] = fma2(decay2(both(s[q]), A[q][0]), h[q][0], mul2(both(x[q]), lo(b4)));
+              h[q][1] = fma2(decay2(both(s[q]), A[q][1]), h[q][1], mul2(both(x[q]), hi(b4)));
               if constexpr (decltype(keep)::value) { H[j][q][0] = h[q][0]; H[j][q][1] = h[q][1]; }
             }
             if (sums) {
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(2 * S::NT, S::LPC <= 2 ? 1 : 2) scan_backward_
               float2 r[2];
 #pragma unroll
               for (int w = 0; w < 2; ++w) {
-                g[q][w] = mul2(g[q][w], exp2_fast(mul2(both(s[q]), A[q][w])));
+                g[q][w] = mul2(g[q][w], decay2(both(s[q]), A[q][w]));
                 r[w] = mul2(g[q][w], j > 0 ? H[j > 0 ? j - 1 : 0][q][w] : before[q][w]);
                 dA[q][w] = fma2(r[w], both(s[q]), dA[q][w]);
               }
