@@ -7,7 +7,7 @@
 //
 // Weights are integers, w * 2^shift: their sums are exact whatever the order of the atomics, and the same draw is made every
 // time.  A draw from 1e5 words goes through as many borders, so a weight good to 24 bits would move a token of every few
-// hundred rows; these are good to 2^-44 or better.  2^t is a table of 2^(k / 256) times the polynomial 1 + r + ... of the rest
+// hundred rows; these are good to 2^-45 of the largest one or better.  2^t is a table of 2^(k / 256) times the polynomial 1 + r + ... of the rest
 // |r| < 2^-9.5 (its first term left out is below 2^-54), in 64-bit floating point, which this chip does at half the 32-bit rate.
 //
 // A cluster of up to eight blocks takes a row, each keeps its slice in shared memory, so the row is read from memory once whatever
@@ -668,8 +668,8 @@ template <typename T, bool RES> cudaError_t launch(const myea_sampling &a, int p
 }
 
 template <typename T> cudaError_t launch(const myea_sampling &a, cudaStream_t stream) {
-  // a slice of some 32 KB leaves room for four blocks on an SM (two of 64 KB measured 220 us where these take 202); more blocks per row while the rows leave SMs idle and a
-  // slice has 4096 words
+  // a slice of some 32 KB leaves room for four blocks on an SM (256 rows of 131072 bf16 words: two of 64 KB took 220 us where these take
+  // 202); more blocks per row while the rows leave SMs idle and a slice has 4096 words
   const uint64_t bytes = a.vocabulary * sizeof(T) + 32;
   int parts = 1;
   while (parts < kParts && (bytes / parts > (36u << 10) || (a.rows * parts * 2 <= 2 * kSms && a.vocabulary / (parts * 2) >= 4096))) parts *= 2;

@@ -318,7 +318,7 @@ ScanArgs arguments(const myea_scan *s) {
   const double blocks = static_cast<double>(a.tiles) * a.groups * a.batch;
   a.chunks = 1;
   a.chunk = (a.time + TT - 1) / TT * TT;
-  if (blocks < kSms * 2 / 3 && a.time >= 8 * TT) {
+  if (blocks > 0 && blocks < kSms * 2 / 3 && a.time >= 8 * TT) {
     const int want = static_cast<int>(4 * kSms / blocks), most = a.time / (4 * TT);
     const int chunks = want < most ? want : most;
     a.chunk = ((a.time + chunks - 1) / chunks + TT - 1) / TT * TT;

@@ -121,3 +121,12 @@ def test_distillation_refusals(change, word):
 def test_sampling_refusals(change, word):
     assert word in refused("sample", sampling(**change))
     assert refused("sample", None) and refused("distillation_error", None)
+
+
+def test_an_empty_batch_needs_little_memory_however_long_its_time():
+    """no sequences of many positions: nothing is cut, and only the (empty) sums of the parameters are formed"""
+    for time in (0, 127, 128, 4096):
+        s = scan(batch=0, time=time)
+        assert capi.load().myea_b200_selective_scan_workspace(C.byref(s)) == 0
+        assert capi.load().myea_b200_selective_scan_backward_workspace(C.byref(s)) == 0
+        assert capi.load().myea_b200_causal_convolution_backward_workspace(C.byref(convolution(batch=0, time=time))) == 0
