@@ -59,7 +59,7 @@ struct alignas(16) Shared {
   // A histogram: words, and their weights in parts of 16, 16 and more bits (RES: sums of up to 65536 words do not carry), or as the
   // 64 bits of the first two.  Afterwards: the words of the bin that holds the limit.
   unsigned int count[kBins], mass[3][kBins];
-  double table[256];                                    // 2^(k / 256)
+  double table[256];                                    // 2^(shift + k / 256)
   u64 warp[kWarps];
   float warp_m[kWarps];
   float m;
@@ -91,6 +91,9 @@ template <typename T, bool RES> struct Draw {
   double md, per;      // 256 log2(e) / temperature
   int shift;
   float beyond;        // distances from here on weigh nothing
+  float lowest;        // words below it weigh nothing
+  bool steep;          // the word below m, or one that is not finite, may be too far off for the arithmetic:
+  double least_d;      // differences are limited to this
   u64 warps[4], upto_warps;   // of total(): up to four warps' sums, and the running sum up to them
 
   __device__ __forceinline__ Draw(Shared &s_) : cluster(cg::this_cluster()), s(s_) {}
@@ -125,20 +128,21 @@ template <typename T, bool RES> struct Draw {
     }
   }
   __device__ __forceinline__ float distance(float e) const { return (0.5f * m - 0.5f * e) * half_scale; }
-  // the weight of a word as an integer; no branches, so that the weights of neighbours are under way together
+  // The weight of a word as an integer.  Most of it is 64-bit floating point, since selects and shifts of 64-bit integers cost more: the
+  // rounding to an integer is the addition of 2^52, and words so far off that they round to 0, closed ones among them, stand for one
+  // that just does.
   __device__ __forceinline__ u64 weight(float e) const {
-    constexpr double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's lower bits are the nearest integer
+    constexpr double magic = 6755399441055744.0, whole = 4503599627370496.0;   // 1.5 * 2^52: the sum's lower bits are the nearest integer; 2^52
     constexpr double c1 = kLn2 / 256, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6, c4 = c1 * c1 * c1 * c1 / 24;
-    const double d = static_cast<double>(e) - md;
+    double d = static_cast<double>(fmaxf(e, lowest)) - md;
+    if (steep) d = e == m ? 0.0 : fmax(d, -least_d);
     const double z = fma(d, per, magic);
     const int i = __double2loint(z);
     const double r = fma(d, per, magic - z);
     double q = fma(fma(fma(fma(r, c4, c3), r, c2), r, c1), r, 1.0);
     q *= s.table[i & 255];
-    const u64 bits = static_cast<u64>(__double_as_longlong(q));
-    const int right = 52 - (static_cast<int>(bits >> 52) - 1023) - (i >> 8) - shift;   // (q > 0; i <= 0)
-    const u64 w = ((bits & ((1ull << 52) - 1)) | (1ull << 52)) >> (right & 63);
-    return e == m ? 1ull << shift : distance(e) < beyond && right < 64 && m != INFINITY ? w : 0;
+    q = __hiloint2double(__double2hiint(q) + static_cast<int>(static_cast<unsigned>(i) << 12 & 0xfff00000u), __double2loint(q)) + whole;   // (times 2^(i >> 8))
+    return static_cast<u64>(__double_as_longlong(q)) & ((1ull << 52) - 1);
   }
   // f(word, its index) for this warp's words from `least` up, lanes side by side; vectors without one are passed over
   template <typename F> __device__ __forceinline__ void each(float least, F f) const {
@@ -159,7 +163,7 @@ template <typename T, bool RES> struct Draw {
     for (int k = 16; k > 0; k >>= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
     return y;
   }
-  // Sums of f over the row's words from `least` up by warps (put into s.warp): their total, in every block
+  // Sums of f, which is 0 below `least`, over the row's words by warps (put into s.warp): their total, in every block
   template <typename F> __device__ u64 total(float least, F f) {
     u64 sum = 0;
     for (int v = from + lane; v < to; v += 32) {
@@ -170,7 +174,7 @@ template <typename T, bool RES> struct Draw {
       for (int h = 0; h < E; h += 4) {   // four chains of arithmetic at a time
         const float4 e = words4(p, h);
         y[h] = f(e.x, v * E + h - lead); y[h + 1] = f(e.y, v * E + h + 1 - lead); y[h + 2] = f(e.z, v * E + h + 2 - lead); y[h + 3] = f(e.w, v * E + h + 3 - lead);
-        sum += (e.x >= least ? y[h] : 0) + (e.y >= least ? y[h + 1] : 0) + (e.z >= least ? y[h + 2] : 0) + (e.w >= least ? y[h + 3] : 0);
+        sum += (y[h] + y[h + 1]) + (y[h + 2] + y[h + 3]);
       }
     }
     sum = warp_sum(sum);
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
         m = fmaxf(m, largest(p[u].v, T()));
       }
   }
-  s.table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 256.0);
+  s.table[threadIdx.x] = ldexp(exp2(static_cast<double>(threadIdx.x) / 256.0), shift);
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   if (d.lane == 0) s.warp_m[d.warp] = m;
@@ -601,9 +605,13 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
   d.m = m;
   d.md = static_cast<double>(m);
   d.half_scale = 2.f / temperature;
-  d.per = 256.0 * kLog2e64 / static_cast<double>(temperature);
+  d.per = fmax(256.0 * kLog2e64 / static_cast<double>(temperature), 1e-300);
   d.shift = shift;
   d.beyond = static_cast<float>((shift + 1) * kLn2) + 0.5f;
+  d.least_d = 256.0 * (shift + 2) / d.per;
+  d.lowest = __double2float_rd(__dadd_rd(d.md, -d.least_d));   // (below m whatever is rounded off)
+  d.steep = !(d.md - static_cast<double>(d.lowest) <= 2.0 * d.least_d);   // (too coarse a float for the distance, or an infinity)
+  if (d.steep) d.lowest = -INFINITY;
 
   Kept kept;
 #pragma unroll 1
@@ -617,15 +625,22 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
     least = min_p >= 1.f ? 1ull << shift : static_cast<u64>(ceil(ldexp(static_cast<double>(min_p), shift)));
     reach = fminf(reach, -logf(min_p) * 1.0001f + 1e-3f);
   }
-  const auto weigh = [&](float e, int i) -> u64 {
-    const u64 w = d.weight(e);
-    return kept.has(e, i) && w >= least ? w : 0;
-  };
   const float nearest = fmaxf(m - reach * 1.001f * temperature, fmaxf(kept.value, -3.402823466e38f));
-  const u64 total = d.total(nearest, weigh);
-  u64 target = uniform > 0.f ? static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(total)) : 0;
-  if (target >= total) target = total - 1;
-  d.find(nearest, target, weigh);
+  u64 total = 0;
+  const auto draw = [&](auto weigh) {
+    total = d.total(nearest, weigh);
+    u64 target = uniform > 0.f ? static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(total)) : 0;
+    if (target >= total) target = total - 1;
+    d.find(nearest, target, weigh);
+  };
+  if (kept.value == -INFINITY && least == 1) {   // nothing is left out
+    draw([&](float e, int) -> u64 { return d.weight(e); });
+  } else {
+    draw([&](float e, int i) -> u64 {
+      const u64 w = d.weight(e);
+      return kept.has(e, i) && w >= least ? w : 0;
+    });
+  }
   d.cluster.sync();
   if (d.part == 0 && threadIdx.x == 0) {
     a.tokens[row] = s.found;

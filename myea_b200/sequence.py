@@ -24,6 +24,8 @@ _DISTILLATION = struct.Struct("<2I3Q" + 3 * "Qq" + "2Q4f2Qq")
 _SAMPLING = struct.Struct("<2I2QQq7Q")
 _NO_VIEW = (0, 0, 0)
 _local = threading.local()   # .message: where the library says why
+# a stream's handle without the object around it (1.3 us of a call's 12)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _call(name, index, *args):
@@ -31,7 +33,7 @@ def _call(name, index, *args):
         message = _local.message
     except AttributeError:
         message = _local.message = C.create_string_buffer(256)
-    rc = getattr(capi.load(), name)(index, *args, torch.cuda.current_stream(index).cuda_stream, message, 256)
+    rc = getattr(capi.load(), name)(index, *args, _stream(index), message, 256)
     if rc != 0:
         raise RuntimeError("%s failed (%d): %s" % (name, rc, message.value.decode()))
 
