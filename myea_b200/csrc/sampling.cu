@@ -22,7 +22,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kParts = 8, kList = 1024;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kParts = 8, kList = 1024, kLongRow = 32;
 static_assert(kThreads == 256, "a thread makes one entry of the table");
 constexpr double kLog2e64 = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
@@ -94,6 +94,7 @@ template <typename T, bool RES> struct Draw {
   float lowest;        // words below it weigh nothing
   bool steep;          // the word below m, or one that is not finite, may be too far off for the arithmetic:
   double least_d;      // differences are limited to this
+  float own;           // the largest word of this thread
   u64 warps[4], upto_warps;   // of total(): up to four warps' sums, and the running sum up to them
 
   __device__ __forceinline__ Draw(Shared &s_) : cluster(cg::this_cluster()), s(s_) {}
@@ -253,76 +254,76 @@ template <typename T, bool RES> struct Draw {
     }
   }
 
-  // Histogram of the words from `least` up for which bin(word, index) >= 0, over the cluster, and the bin that holds the limit: the first, from bin 0
-  // on, with `target` words (or `target` of weight) up to its end.  part_of_all < 1: the target is that part of the whole weight.
-  // s.bin is -1 where there is less.  On entry before_count / before_mass: what lies in front of bin 0.
-  template <typename F> __device__ void limit_bin(float least, bool by_mass, double part_of_all, u64 target, u64 before_count, u64 before_mass, F bin) {
-    for (int k = threadIdx.x; k < kBins; k += kThreads) s.count[k] = s.mass[0][k] = s.mass[1][k] = s.mass[2][k] = 0;
-    if (threadIdx.x == 0) { s.bin = -1; s.total_mass = 0; s.listed = 0; }
-    __syncthreads();
-    if (by_mass) {
-      for (int v = from + lane; v < to; v += 32) {
-        const Pack<T> p = words(v);
-        if (!(largest(p.v, T()) >= least)) continue;
-#pragma unroll
-        for (int h = 0; h < E; h += 4) {   // four chains of arithmetic at a time
-          const float4 e4 = words4(p, h);
-          const float e[4] = {e4.x, e4.y, e4.z, e4.w};
-          u64 w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = weight(e[k]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int b = e[k] >= least ? bin(e[k], v * E + h + k - lead) : -1;
-            if (b < 0) continue;
-            atomicAdd(&s.count[b], 1u);
-            if constexpr (RES) {
-              atomicAdd(&s.mass[0][b], static_cast<unsigned>(w[k] & 0xffff));
-              atomicAdd(&s.mass[1][b], static_cast<unsigned>(w[k] >> 16) & 0xffffu);
-              atomicAdd(&s.mass[2][b], static_cast<unsigned>(w[k] >> 32));
-            } else {
-              atomicAdd(reinterpret_cast<u64 *>(s.mass[0]) + b, w[k]);
-            }
-          }
-        }
-      }
-    } else {
+  // Counts the words from `least` up by bin(word, index), those with bin < 0 left out; by_mass: and adds up their weights
+  template <typename F> __device__ __forceinline__ void histogram(float least, bool by_mass, F bin) {
+    if (!by_mass) {
       each(least, [&](float e, int i) {
         const int b = bin(e, i);
         if (b >= 0) atomicAdd(&s.count[b], 1u);
       });
+      return;
     }
+    for (int v = from + lane; v < to; v += 32) {
+      const Pack<T> p = words(v);
+      if (!(largest(p.v, T()) >= least)) continue;
+#pragma unroll
+      for (int h = 0; h < E; h += 4) {   // four chains of arithmetic at a time
+        const float4 e4 = words4(p, h);
+        const float e[4] = {e4.x, e4.y, e4.z, e4.w};
+        u64 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = weight(e[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int b = e[k] >= least ? bin(e[k], v * E + h + k - lead) : -1;
+          if (b < 0) continue;
+          atomicAdd(&s.count[b], 1u);
+          if constexpr (RES) {
+            atomicAdd(&s.mass[0][b], static_cast<unsigned>(w[k] & 0xffff));
+            atomicAdd(&s.mass[1][b], static_cast<unsigned>(w[k] >> 16) & 0xffffu);
+            atomicAdd(&s.mass[2][b], static_cast<unsigned>(w[k] >> 32));
+          } else {
+            atomicAdd(reinterpret_cast<u64 *>(s.mass[0]) + b, w[k]);
+          }
+        }
+      }
+    }
+  }
+  // Makes a histogram by fill(), over the cluster, and finds the bin that holds the limit: the first, from bin 0 on, with `target`
+  // words (or `target` of weight) up to its end.  part_of_all < 1: the target is that part of the whole weight.
+  // s.bin is -1 where there is less.  before_count / before_mass: what lies in front of bin 0.
+  template <typename F> __device__ void limit_bin(bool by_mass, double part_of_all, u64 target, u64 before_count, u64 before_mass, F fill) {
+    for (int k = threadIdx.x; k < kBins; k += kThreads) s.count[k] = s.mass[0][k] = s.mass[1][k] = s.mass[2][k] = 0;
+    if (threadIdx.x == 0) { s.bin = -1; s.total_mass = 0; s.listed = 0; }
+    __syncthreads();
+    fill();
     cluster.sync();
-    constexpr int B = kBins / kThreads;
-    static_assert(B % 4 == 0, "a thread's bins are vectors");
-    u64 c[B], w[B], sum_c = 0, sum_w = 0;
-#pragma unroll
-    for (int k = 0; k < B; ++k) { c[k] = 0; w[k] = 0; }
-    const auto gather = [&](const unsigned *bins, u64 (&to_)[B], int left) {   // (all the blocks' loads under way together)
-#pragma unroll
-      for (int j = 0; j < B; j += 4) {
-#pragma unroll 2
-        for (int o = 0; o < parts; ++o) {
-          const uint4 n = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(bins, o) + threadIdx.x * B + j);
-          to_[j] += static_cast<u64>(n.x) << left; to_[j + 1] += static_cast<u64>(n.y) << left;
-          to_[j + 2] += static_cast<u64>(n.z) << left; to_[j + 3] += static_cast<u64>(n.w) << left;
+    // Every block adds up its share of the bins (all of them in every block took four times as long): one to four neighbouring bins per
+    // thread.
+    const int bins = kBins / parts, each_thread = bins > kThreads ? bins / kThreads : 1, mine = static_cast<int>(threadIdx.x) * each_thread;
+    const int first_bin = part * bins + mine;
+    const auto bin_sums = [&](int k, u64 &c, u64 &w) {   // of bin k, over the blocks
+      c = w = 0;
+#pragma unroll 4
+      for (int o = 0; o < parts; ++o) {
+        const Shared *h = cluster.map_shared_rank(&s, o);
+        c += h->count[k];
+        if (by_mass) {
+          if constexpr (RES) w += h->mass[0][k] + (static_cast<u64>(h->mass[1][k]) << 16) + (static_cast<u64>(h->mass[2][k]) << 32);
+          else w += reinterpret_cast<const u64 *>(h->mass[0])[k];
         }
       }
     };
-    gather(s.count, c, 0);
-    if (by_mass) {
-      if constexpr (RES) {
-        gather(s.mass[0], w, 0);
-        gather(s.mass[1], w, 16);
-        gather(s.mass[2], w, 32);
-      } else {
-        for (int o = 0; o < parts; ++o)
-#pragma unroll
-          for (int k = 0; k < B; ++k) w[k] += reinterpret_cast<const u64 *>(cluster.map_shared_rank(s.mass[0], o))[threadIdx.x * B + k];
+    u64 sum_c = 0, sum_w = 0;
+    if (mine < bins) {
+#pragma unroll 1
+      for (int k = 0; k < each_thread; ++k) {
+        u64 c, w;
+        bin_sums(first_bin + k, c, w);
+        sum_c += c;
+        sum_w += w;
       }
     }
-#pragma unroll
-    for (int k = 0; k < B; ++k) { sum_c += c[k]; sum_w += w[k]; }
     u64 upto_c = sum_c, upto_w = sum_w;
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
@@ -330,35 +331,47 @@ template <typename T, bool RES> struct Draw {
       if (lane >= k) { upto_c += oc; upto_w += ow; }
     }
     if (lane == 31) { s.scan_count[warp] = upto_c; s.scan_mass[warp] = upto_w; }
-    __syncthreads();
-    u64 all_c = 0, all_w = 0;
-    for (int k = 0; k < kWarps; ++k) {
-      if (k < warp) { before_count += s.scan_count[k]; before_mass += s.scan_mass[k]; }
-      all_c += s.scan_count[k];
-      all_w += s.scan_mass[k];
+    cluster.sync();
+    // the sums of all the warps of all the blocks: up to two per lane
+    u64 all_c = 0, all_w = 0, in_front_c = 0, in_front_w = 0;
+    for (int k = lane; k < parts * kWarps; k += 32) {
+      const Shared *h = cluster.map_shared_rank(&s, k / kWarps);
+      const u64 n = h->scan_count[k % kWarps], y = h->scan_mass[k % kWarps];
+      all_c += n;
+      all_w += y;
+      if (k < part * kWarps + warp) { in_front_c += n; in_front_w += y; }
+    }
+    all_c = warp_sum(all_c);
+    before_count += warp_sum(in_front_c) + upto_c - sum_c;
+    if (by_mass) {
+      all_w = warp_sum(all_w);
+      before_mass += warp_sum(in_front_w) + upto_w - sum_w;
     }
     if (part_of_all < 1.0) target = static_cast<u64>(ceil(part_of_all * static_cast<double>(all_w)));
-    before_count += upto_c - sum_c;
-    before_mass += upto_w - sum_w;
-#pragma unroll
-    for (int k = 0; k < B; ++k) {
-      if (c[k] != 0) {
-        // the first bin of words with enough up to its end
-        const bool enough = by_mass ? before_mass + w[k] >= target : before_count + c[k] >= target;
-        const bool was = by_mass ? before_count != 0 && before_mass >= target : before_count >= target;
-        if (enough && !was) {
-          s.bin = threadIdx.x * B + k;
-          s.before_count = before_count;
-          s.before_mass = before_mass;
-          s.bin_count = c[k];
-          s.bin_mass = w[k];
+    // the first bin of words with enough up to its end
+    const bool enough = by_mass ? before_mass + sum_w >= target : before_count + sum_c >= target;
+    const bool was = by_mass ? before_count != 0 && before_mass >= target : before_count >= target;
+    if (sum_c != 0 && enough && !was) {
+      u64 c, w;
+      for (int k = first_bin;; ++k) {
+        bin_sums(k, c, w);
+        if (c != 0 && (by_mass ? before_mass + w >= target : before_count + c >= target)) {
+          for (int o = 0; o < parts; ++o) {
+            Shared *to_ = cluster.map_shared_rank(&s, o);
+            to_->bin = k;
+            to_->before_count = before_count;
+            to_->before_mass = before_mass;
+            to_->bin_count = c;
+            to_->bin_mass = w;
+          }
+          break;
         }
+        before_count += c;
+        before_mass += w;
       }
-      before_count += c[k];
-      before_mass += w[k];
     }
     if (threadIdx.x == 0) { s.total_mass = target; s.all_count = all_c; s.all_mass = all_w; }
-    cluster.sync();   // nobody clears its bins while others read them
+    cluster.sync();   // nobody clears its bins, or writes the next sums, while others read them
   }
 
   // keeps the first `target` words, or those before which less than the part `part_of_all` of the weight of what was kept lies
@@ -366,29 +379,47 @@ template <typename T, bool RES> struct Draw {
     // bins by distance: 32 to a unit, of the logits for counts and of the logarithm of the weights for weights (behind the last
     // bin those weigh nothing: 2^-46)
     const float scale = by_mass ? 32.f * half_scale : 64.f;
+    float fine = 1.f;   // the bins are so many times finer
     const auto far = [&](float e) {
-      const float t = (0.5f * m - 0.5f * e) * scale;
+      const float t = (0.5f * m - 0.5f * e) * scale * fine;
       return e == m ? 0 : t < static_cast<float>(kBins - 1) ? static_cast<int>(t) : kBins - 1;
     };
+    const auto reach_of = [&](float bin) { return (bin + 2.f) * 1.0001f / scale * 2.f; };   // (the words up to that bin, of the first kind, are nearer)
     const Kept was = kept;
     const float lowest_open = fmaxf(was.value, -3.402823466e38f);
+    float least = lowest_open;
+    u64 before_count = 0, before_mass = 0;
+    // Counts in a long row: most words are passed over by a bound that is found first.  So many threads have a word as far up as the
+    // limit, so no word below the last of these counts.
+    if (!by_mass && V >= kLongRow * parts * kThreads && target <= static_cast<u64>(parts) * kThreads) {
+      limit_bin(false, 1.0, target, 0, 0, [&]() {
+        const int b = own > -INFINITY ? far(own) : kBins - 1;
+        if (b < kBins - 1) atomicAdd(&s.count[b], 1u);
+      });
+      const int bin = s.bin;
+      if (bin >= 0) {
+        least = fmaxf(least, m - reach_of(bin));
+        fine = static_cast<float>(kBins - 2) / ((static_cast<float>(bin) + 2.f) * 1.001f + 1.f);
+      }
+      __syncthreads();
+    }
     // Counts beyond the last bin are taken only when the limit lies there: most words of a row may, and their additions to one bin
     // would wait for one another.
-    float least = lowest_open;
     bool by_distance = true;
     int bin = 0, narrow = 0;
     uint32_t lo = 0, hi = 0, lowest = 0xffffffffu, highest = 0;
-    u64 before_count = 0, before_mass = 0;
 #pragma unroll 1
     while (true) {
-      limit_bin(least, by_mass, by_distance && by_mass ? part_of_all : 1.0, target, before_count, before_mass, [&](float e, int i) {
-        if (!was.has(e, i)) return -1;
-        if (by_distance) {
-          const int b = far(e);
-          return b < kBins - 1 ? b : -1;
-        }
-        const uint32_t k = key_of(e);
-        return k >= lo && k <= hi ? static_cast<int>((hi - k) >> narrow) : -1;
+      limit_bin(by_mass, by_distance && by_mass ? part_of_all : 1.0, target, before_count, before_mass, [&]() {
+        histogram(least, by_mass, [&](float e, int i) {
+          if (!was.has(e, i)) return -1;
+          if (by_distance) {
+            const int b = far(e);
+            return b < kBins - 1 ? b : -1;
+          }
+          const uint32_t k = key_of(e);
+          return k >= lo && k <= hi ? static_cast<int>((hi - k) >> narrow) : -1;
+        });
       });
       const int at = s.bin;
       before_count = at < 0 ? s.all_count : s.before_count;
@@ -408,8 +439,7 @@ template <typename T, bool RES> struct Draw {
           if (by_mass) return;
           bin = kBins - 1;
         } else {
-          const float reach = static_cast<float>(bin + 2) * 1.0001f / scale * 2.f;   // (the bin's words are nearer than this)
-          least = fmaxf(least, m - reach);
+          least = fmaxf(least, m - reach_of(static_cast<float>(bin + 1) / fine));
         }
         if (bin < kBins - 1 && s.bin_count <= kList) {   // few words in the bin: the first block sorts them
           Shared *head = cluster.map_shared_rank(&s, 0);
@@ -578,6 +608,7 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
         m = fmaxf(m, largest(p[u].v, T()));
       }
   }
+  d.own = m;
   s.table[threadIdx.x] = ldexp(exp2(static_cast<double>(threadIdx.x) / 256.0), shift);
 #pragma unroll
   for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
@@ -635,6 +666,11 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
   };
   if (kept.value == -INFINITY && least == 1) {   // nothing is left out
     draw([&](float e, int) -> u64 { return d.weight(e); });
+  } else if (least == 1) {
+    draw([&](float e, int i) -> u64 {
+      const u64 w = d.weight(e);
+      return kept.has(e, i) ? w : 0;
+    });
   } else {
     draw([&](float e, int i) -> u64 {
       const u64 w = d.weight(e);
