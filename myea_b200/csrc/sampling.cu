@@ -10,6 +10,10 @@
 // hundred rows; these are good to 2^-45 of the largest one or better.  2^t is a table of 2^(k / 256) times the polynomial 1 + r + ... of the rest
 // |r| < 2^-9.5 (its first term left out is below 2^-54), in 64-bit floating point, which this chip does at half the 32-bit rate.
 //
+// Bound by instructions and, with rows for fewer than two waves of blocks, by a row's chain of passes: 256 rows of 131072 bf16 words take
+// 30 us for the largest word alone (2.2 TB/s), 83 for a draw from all words, 118 from the 50 best, 275 from top-p 0.9.  A bound from a
+// sample for top-p, too, left out most additions to bins, but its code cost more (335 us).
+//
 // A cluster of up to eight blocks takes a row, each keeps its slice in shared memory, so the row is read from memory once whatever
 // is asked of it; rows beyond the clusters' memory are read again in every pass.  A warp works on a contiguous part of a slice, so
 // that the draw, which goes by rising index, finds its word from the warps' sums and one warp's walk over its part.
@@ -390,7 +394,8 @@ template <typename T, bool RES> struct Draw {
     float least = lowest_open;
     u64 before_count = 0, before_mass = 0;
     // Counts in a long row: most words are passed over by a bound that is found first.  So many threads have a word as far up as the
-    // limit, so no word below the last of these counts.
+    // limit, so no word below the last of these counts.  (With 16 words per thread the second histogram costs what the bound saves, 19 us
+    // for a row of 32000; with 128, 256 rows of 131072 take 118 us in place of 143.)
     if (!by_mass && V >= kLongRow * parts * kThreads && target <= static_cast<u64>(parts) * kThreads) {
       limit_bin(false, 1.0, target, 0, 0, [&]() {
         const int b = own > -INFINITY ? far(own) : kBins - 1;
@@ -719,8 +724,8 @@ template <typename T, bool RES> cudaError_t launch(const myea_sampling &a, int p
 }
 
 template <typename T> cudaError_t launch(const myea_sampling &a, cudaStream_t stream) {
-  // a slice of some 32 KB leaves room for four blocks on an SM (256 rows of 131072 bf16 words: two of 64 KB took 220 us where these take
-  // 202); more blocks per row while the rows leave SMs idle and a slice has 4096 words
+  // A slice of some 32 KB leaves room for four blocks on an SM (256 rows of 131072 bf16 words: two of 64 KB took a tenth longer).  More
+  // blocks per row while the rows leave SMs idle and a slice has 4096 words.
   const uint64_t bytes = a.vocabulary * sizeof(T) + 32;
   int parts = 1;
   while (parts < kParts && (bytes / parts > (36u << 10) || (a.rows * parts * 2 <= 2 * kSms && a.vocabulary / (parts * 2) >= 4096))) parts *= 2;
