@@ -6,6 +6,8 @@
 // read from memory once; the W - 1 positions that neighbouring runs share come out of L2.  What holds it back is the number of warps
 // that fit beside such registers: 4 x 2048 x 4096 bf16 with 4 taps take 48 us forward (2.8 TB/s) and 81 us backward; two
 // blocks per SM instead of three 52 us, one instead of two 122 us.
+#include <math.h>
+
 #include "sequence.cuh"
 
 namespace myea {
@@ -240,12 +242,23 @@ __global__ void __launch_bounds__(256) convolution_finish_kernel(const float *pa
   sum_partials_block(part, rows, columns, blockIdx.x, store);
 }
 
-// A run's positions: long ones read little twice, short ones give a small batch its threads (148 SMs x 1024)
-int run_length(uint64_t batch, uint64_t time, uint64_t width) {
-  const uint64_t per_position = batch * ((width + 3) / 4);
-  for (int run = 32; run > 8; run /= 2)
-    if (per_position * ((time + run - 1) / run) >= uint64_t(kSms) * 1024) return run;
-  return 8;
+// A run's positions: the launch takes as long as its waves of blocks, each as long as a run, the positions that a run reads twice and
+// what a thread does once (together some 8 positions).  4 x 2048 x 4096: 80 forward and 128 backward, one wave each.
+int run_length(const myea_convolution *c, bool backward) {
+  const int64_t resident = kSms * (c->taps > 4 ? 1 : backward ? 2 : 3), batch = static_cast<int64_t>(c->batch), time = static_cast<int64_t>(c->time);
+  const int64_t groups = (static_cast<int64_t>(c->width) + 3) / 4;
+  int best = 8;
+  double least = 1e300;
+  for (int run = 8; run <= 128; run += 4) {
+    const int64_t runs = (time + run - 1) / run;
+    const double blocks = backward ? static_cast<double>((groups + 31) / 32) * ((runs + 7) / 8) * batch : static_cast<double>(groups) * runs * batch / 256;
+    const double cost = ceil(blocks / resident) * (run + 8);
+    if (cost < least) {
+      least = cost;
+      best = run;
+    }
+  }
+  return best;
 }
 
 const char *check(const myea_convolution *c, bool backward) {
@@ -268,12 +281,12 @@ const char *check(const myea_convolution *c, bool backward) {
   return nullptr;
 }
 
-ConvArgs arguments(const myea_convolution *c) {
+ConvArgs arguments(const myea_convolution *c, bool backward) {
   ConvArgs s = {};
   s.c = *c;
   s.batch = static_cast<int>(c->batch); s.time = static_cast<int>(c->time); s.width = static_cast<int>(c->width);
   s.vectors = (s.width + 3) / 4;
-  s.run = run_length(c->batch, c->time, c->width);
+  s.run = run_length(c, backward);
   s.runs = s.time > 0 ? (s.time + s.run - 1) / s.run : 1;
   const size_t bytes = 4 * type_bytes(c->type);
   const bool even = c->width % 4 == 0;
@@ -314,7 +327,7 @@ extern "C" int myea_b200_causal_convolution(int device, const myea_convolution *
   using namespace myea;
   if (const char *why = check(c, false)) return refuse(error_message, error_capacity, MYEA_E_INVALID, why);
   if (c->batch == 0 || c->width == 0) return MYEA_OK;
-  const ConvArgs s = arguments(c);
+  const ConvArgs s = arguments(c, false);
   const long long blocks = (static_cast<long long>(s.vectors) * s.runs * s.batch + 255) / 256;
   if (s.vectors > (1ll << 62) / (static_cast<long long>(s.runs) * s.batch) || blocks > 0x7fffffffll)
     return refuse(error_message, error_capacity, MYEA_E_INVALID, "causal_convolution: more positions than one launch takes");
@@ -328,7 +341,7 @@ extern "C" int myea_b200_causal_convolution(int device, const myea_convolution *
 extern "C" size_t myea_b200_causal_convolution_backward_workspace(const myea_convolution *c) {
   using namespace myea;
   if (check(c, true) != nullptr || c->batch == 0 || c->width == 0 || (c->d_weight == nullptr && c->d_bias == nullptr)) return 0;
-  const ConvArgs s = arguments(c);
+  const ConvArgs s = arguments(c, true);
   return round_up_256(c->batch * run_blocks_of(s) * (c->taps + 1) * c->width * sizeof(float));
 }
 
@@ -340,7 +353,7 @@ extern "C" int myea_b200_causal_convolution_backward(int device, const myea_conv
   const size_t need = myea_b200_causal_convolution_backward_workspace(c);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)))
     return refuse(error_message, error_capacity, MYEA_E_INVALID, "causal_convolution: the workspace is missing, too small or not 256-byte aligned");
-  ConvArgs s = arguments(c);
+  ConvArgs s = arguments(c, true);
   s.partial = need > 0 ? static_cast<float *>(workspace) : nullptr;
   const int tiles = (s.vectors + 31) / 32, run_blocks = run_blocks_of(s);
   const double blocks_wide = static_cast<double>(tiles) * run_blocks * s.batch;
