@@ -4,8 +4,9 @@
 // Bound by memory: a handful of multiply-adds per element.  A thread takes four channels (8 or 16 bytes) over a run of
 // positions and keeps the last W inputs, and backward the W errors that are not complete yet, in registers, so each element is
 // read from memory once; the W - 1 positions that neighbouring runs share come out of L2.  What holds it back is the number of warps
-// that fit beside such registers: 4 x 2048 x 4096 bf16 with 4 taps take 48 us forward (2.8 TB/s) and 81 us backward; two
-// blocks per SM instead of three 52 us, one instead of two 122 us.
+// that fit beside such registers: 4 x 2048 x 4096 bf16 with 4 taps take 40 us forward (3.4 TB/s) and 73 us backward (2.8 TB/s).
+// Measured with shorter runs: two blocks per SM instead of three 52 us for 48, backward one instead of two 122 us for 81.  Loads
+// eight positions ahead instead of four 38 us, but 4.4 us in place of 3.7 for single positions of 64 sequences.
 #include <math.h>
 
 #include "sequence.cuh"
