@@ -502,7 +502,7 @@ int myea_b200_distillation_error(int device, const myea_distillation *d, void *s
  * index: the first whose running sum of w exceeds uniform * (their sum).  temperature <= 0: the largest logit, the lowest index where several
  * are.  Settings are arrays of one value per row; null: temperature 1, no limit.  Minus infinity and NaN are closed words; a row
  * without any other has token -1 and chance 0.  Words of plus infinity share the draw alone.  chances (may be null): w / sum of the token.
- * Weights are summed as integers, so that the draw does not depend on the order of summation: each is cut to a multiple of 2^-k of the
+ * Weights are summed as integers, so that the draw does not depend on the order of summation: each is rounded to a multiple of 2^-k of the
  * row's largest one, k = 62 less the bits that count the vocabulary (45 for 131072 words) and at most 51; for top_p weights below
  * 2^-46 of it count as nothing. */
 typedef struct myea_sampling {

@@ -99,6 +99,11 @@ def _workspace(name, description, like):
     return work, work.data_ptr(), size
 
 
+def _empty_like(x):
+    """a densely packed tensor of x's shape and type"""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)   # (the first is quicker)
+
+
 def causal_convolution(x, weight, bias=None, silu=True, state=None, final_state=None, lengths=None, out=None):
     """(y, final_state): y[b, t, c] = act(bias[c] + sum over j of weight[c, j] * x[b, t - taps + 1 + j, c]), act = silu or nothing.
     weight [width, taps], 1 to 8 taps; state [batch, taps - 1, width]: the inputs before the first (None: zeros); final_state: where the
@@ -110,7 +115,7 @@ def causal_convolution(x, weight, bias=None, silu=True, state=None, final_state=
     (b, t, d), k, tp, at = x.shape, weight.shape[1], x.dtype, x.get_device()
     whole, before = (b, t, d), (b, k - 1, d)
     if out is None:
-        out = x.new_empty(whole)
+        out = _empty_like(x)
     if final_state is None:
         final_state = x.new_empty(before)
     _call("myea_b200_causal_convolution", at, _CONVOLUTION.pack(
@@ -130,7 +135,7 @@ def causal_convolution_backward(dy, x, weight, bias=None, silu=True, state=None,
     (b, t, d), k, tp, at = x.shape, weight.shape[1], x.dtype, x.get_device()
     whole, before = (b, t, d), (b, k - 1, d)
     if dx is None:
-        dx = x.new_empty(whole)
+        dx = _empty_like(x)
     d_weight = _gradient("d_weight", d_weight, (d, k), x, accumulate)
     d_bias = _gradient("d_bias", d_bias, (d,), x, accumulate) if bias is not None else None
     d_state = x.new_empty(before) if state is not None else None
@@ -180,9 +185,9 @@ def selective_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, softplus
     time = 1 with both states."""
     kind, (b, t, d, n, g), at, views, arrays, lengths_at = _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths)
     if out is None:
-        out = u.new_empty((b, t, d))
+        out = _empty_like(u)
     if final_state is None:
-        final_state = u.new_empty((b, d, n), dtype=_F32)
+        final_state = u.new_empty((b, d, n), dtype=_F32) if state is None else torch.empty_like(state)
     kept = 0 if checkpoints is None else _array("checkpoints", checkpoints, _checkpoint_shape(b, t, d, n), _F32, at)
     s = _SCAN.pack(kind, 1 if softplus else 0, 0, 0, b, t, d, n, g, *views, *_view("out", out, (b, t, d), u.dtype, at), *arrays,
                    _array("final_state", final_state, (b, d, n), _F32, at), lengths_at, kept, *_NO_GRADIENTS)
@@ -201,7 +206,7 @@ def selective_scan_backward(dy, u, delta, A, B, C_, checkpoints, D=None, z=None,
     there, with `accumulate` onto what they hold."""
     kind, (b, t, d, n, g), at, views, arrays, lengths_at = _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths)
     tp, whole, narrow, held = u.dtype, (b, t, d), (b, t, g, n), (b, d, n)
-    got = {"u": u.new_empty(whole), "delta": u.new_empty(whole), "B": u.new_empty(narrow), "C": u.new_empty(narrow), "z": u.new_empty(whole) if z is not None else None,
+    got = {"u": _empty_like(u), "delta": _empty_like(u), "B": u.new_empty(narrow), "C": u.new_empty(narrow), "z": _empty_like(u) if z is not None else None,
            "A": _gradient("d_A", d_A, (d, n), u, accumulate), "D": _gradient("d_D", d_D, (d,), u, accumulate) if D is not None else None,
            "delta_bias": _gradient("d_delta_bias", d_delta_bias, (d,), u, accumulate) if delta_bias is not None else None,
            "state": u.new_empty(held, dtype=_F32) if state is not None else None}
@@ -241,7 +246,7 @@ def distillation_error(logits, index, teacher, temperature=1.0, soft=1.0, hard=0
     if not derivatives:
         d_logits = None
     elif d_logits is None:
-        d_logits = logits.new_empty((r, v))
+        d_logits = _empty_like(logits)
     _call("myea_b200_distillation_error", at, _DISTILLATION.pack(
         kind, 0, r, v, k, *_rows("logits", logits, (r, v), tp, at), *_rows("index", index, (r, k), _I32, at), *_rows("teacher", teacher, (r, k), _F32, at),
         _array("labels", labels, (r,), _I32, at), _array("weight", weight, (r,), _F32, at), temperature, soft, hard, 0.0,
@@ -261,7 +266,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     if tokens is None:
         tokens = logits.new_empty(one, dtype=_I32)
     if chances is None:
-        chances = logits.new_empty(one, dtype=_F32)
+        chances = torch.empty_like(uniform) if uniform is not None else logits.new_empty(one, dtype=_F32)
     _call("myea_b200_sample", at, _SAMPLING.pack(
         kind, 0, r, v, *_rows("logits", logits, (r, v), logits.dtype, at), _array("uniform", uniform, one, _F32, at), _array("temperature", temperature, one, _F32, at),
         _array("top_k", top_k, one, _I32, at), _array("top_p", top_p, one, _F32, at), _array("min_p", min_p, one, _F32, at),

@@ -172,3 +172,27 @@ def test_calls_side_by_side():
         for got in results[k]:
             for a, b in zip(got, alone[k]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["normal", "sorted", "steps", "closed", "peaked", "flat"])
+def test_limits_of_long_rows(kind):
+    """limits about the number of threads that a row has, and words of which every thread, few threads or one have the largest"""
+    v, gen = 131072, torch.Generator(device=DEV).manual_seed(50)
+    x = torch.randn(6, v, generator=gen, device=DEV) * 2
+    if kind == "sorted":
+        x = x.sort(1)[0]
+    if kind == "steps":
+        x = x.round()
+    if kind == "closed":
+        x[torch.rand(6, v, generator=gen, device=DEV) < 0.995] = -math.inf
+    if kind == "peaked":
+        x[:, v // 3] += 30.0
+    if kind == "flat":
+        x = torch.full_like(x, 1.5)
+    u = torch.rand(6, generator=gen, device=DEV)
+    top_k = torch.tensor([1, 1023, 2047, 2048, 2049, v - 1], dtype=torch.int32, device=DEV)
+    top_p = torch.tensor([0.5, 0.9, 0.999, 0.01, 0.7, 0.95], device=DEV)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype)
+        check_sampling(y, u, top_k=top_k)
+        check_sampling(y, u, torch.full((6,), 0.6, device=DEV), top_k, top_p)
