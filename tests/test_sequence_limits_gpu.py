@@ -196,3 +196,42 @@ def test_limits_of_long_rows(kind):
         y = x.to(dtype)
         check_sampling(y, u, top_k=top_k)
         check_sampling(y, u, torch.full((6,), 0.6, device=DEV), top_k, top_p)
+
+
+def test_a_captured_token_step_carries_its_states():
+    """a step of answering in one graph, the states written in place and its logits scored against a teacher, replayed on new inputs"""
+    b, d, n = 5, 200, 16
+    gen = torch.Generator(device=DEV).manual_seed(60)
+    w, bias, A = normal(gen, d, 4), normal(gen, d), -torch.exp(normal(gen, d, n))
+    index, teacher = teacher_for(gen, b, d, 7)
+    top_p = torch.full((b,), 0.8, device=DEV)
+    inputs = [dict(x=normal(gen, b, 1, d), z=normal(gen, b, 1, d), delta=normal(gen, b, 1, d), B=normal(gen, b, 1, 1, n), C=normal(gen, b, 1, 1, n),
+                   u=torch.rand(b, generator=gen, device=DEV)) for _ in range(4)]
+    start = [normal(gen, b, 3, d), normal(gen, b, d, n)]
+
+    def step(i, conv, h):
+        x, _ = sequence.causal_convolution(i["x"], w, bias, state=conv, final_state=conv)
+        y, _ = sequence.selective_scan(x, i["delta"], A, i["B"], i["C"], z=i["z"], state=h, final_state=h)
+        tokens, chances = sequence.sample(y[:, 0], i["u"], top_p=top_p)
+        losses, grad = sequence.distillation_error(y[:, 0], index, teacher, temperature=2.0)
+        return [y, tokens, chances, losses, grad]
+
+    conv, h = (s.clone() for s in start)
+    want = [[v.clone() for v in step(i, conv, h)] + [conv.clone(), h.clone()] for i in inputs]
+    held, states = {k: v.clone() for k, v in inputs[0].items()}, [s.clone() for s in start]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held, *states)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held, *states)
+    for s, v in zip(states, start):
+        s.copy_(v)
+    for i, expected in zip(inputs, want):
+        for k, v in i.items():
+            held[k].copy_(v)
+        graph.replay()
+        for a, e in zip(out + states, expected):
+            assert torch.equal(a, e)
