@@ -8,6 +8,8 @@
 // time out of L2: 296 rows of 256 KB at a time fit there as long as the gradients, which nobody reads here, are stored past it
 // (stored the ordinary way a third of the second reading came out of memory again).  2048 rows of 131072 bf16 logits: 252 us, 4.3 TB/s
 // of 6.5; a block of 1024 threads per SM 272 us, registers of clusters of four 422 us, most of it waiting for one another.
+// Many short rows are bound by a row's chain of steps, so as many blocks as can be lie side by side: 4096 rows of 1024 fp32 logits
+// 18.3 us with 40 registers a thread, 19.3 with 54, 20.8 as clusters of one block, 28 with a warp per row.
 // A cluster of blocks takes a row only where the rows leave SMs idle; the blocks' parts of the sums are exchanged through
 // shared memory and joined in rank order.
 // Exponents are formed from x - m, which is exact near the maximum, where it counts.  The first warp
@@ -83,7 +85,7 @@ struct Running {
 
 // P: packs of a thread at a time
 template <typename T, bool TWO, int P>
-__global__ void __launch_bounds__(512, 2) distillation_kernel(const myea_distillation d) {
+__global__ void __launch_bounds__(512, P == 2 ? 3 : 2) distillation_kernel(const myea_distillation d) {
   constexpr int E = Pack<T>::N;
   extern __shared__ float dynamic[];
   int *s_index = reinterpret_cast<int *>(dynamic);
@@ -312,7 +314,7 @@ template <typename T, int P> cudaError_t launch(const myea_distillation &d, int 
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   const bool two = d.hard != 0.f && d.temperature != 1.f && d.labels != nullptr;
   return two ? cudaLaunchKernelEx(&cfg, distillation_kernel<T, true, P>, d) : cudaLaunchKernelEx(&cfg, distillation_kernel<T, false, P>, d);
 }

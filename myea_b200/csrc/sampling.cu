@@ -719,7 +719,7 @@ template <typename T, bool RES> cudaError_t launch(const myea_sampling &a, int p
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, sampling_kernel<T, RES>, a, shift_for(a.vocabulary));
 }
 
