@@ -235,3 +235,15 @@ def test_a_captured_token_step_carries_its_states():
         graph.replay()
         for a, e in zip(out + states, expected):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype,r,v", [(torch.bfloat16, 1200, 2500), (torch.float32, 300, 2305), (torch.float16, 300, 16003), (torch.bfloat16, 203, 32001),
+                                       (torch.bfloat16, 320, 33003), (torch.float32, 1200, 700)])
+def test_distillation_by_rows_and_lengths(dtype, r, v):
+    """numbers of rows and lengths between which the threads of a row change"""
+    gen = torch.Generator(device=DEV).manual_seed(v)
+    x = (torch.randn(r, v, generator=gen, device=DEV) * 3).to(dtype)
+    index, teacher = teacher_for(gen, r, v, 6)
+    labels = torch.randint(v, (r,), generator=gen, device=DEV, dtype=torch.int32)
+    check_distillation(x, index, teacher, 1.5, 0.5, 0.5, labels, torch.rand(r, generator=gen, device=DEV))
+    check_distillation(x, index, teacher, in_place=True)
