@@ -498,8 +498,8 @@ int myea_b200_distillation_error(int device, const myea_distillation *d, void *s
 /* One token for every row of `logits`, drawn with the given random number (uniform[row] in [0, 1)), beside the output layer's
  * values.  With m the row's largest logit, w[i] = exp((logits[i] - m) / temperature[row]), tokens ordered by falling logit and, where
  * these are equal, rising index:  top_k > 0 keeps the first top_k;  top_p < 1 keeps of these every token before which less than
- * top_p of their sum of w lies, and the first in any case;  min_p > 0 keeps what has w >= min_p.  The draw goes through the kept tokens by rising
- * index: the first whose running sum of w exceeds uniform * (their sum).  temperature <= 0: the largest logit, the lowest index where several
+ * top_p of their sum of w lies, and the first in any case;  min_p > 0 keeps what has w >= min_p, min_p above 1 counting as 1.  The draw goes through the kept
+ * tokens by rising index: the first whose running sum of w exceeds uniform * (their sum).  temperature <= 0: the largest logit, the lowest index where several
  * are.  Settings are arrays of one value per row; null: temperature 1, no limit.  Minus infinity and NaN are closed words; a row
  * without any other has token -1 and chance 0.  Words of plus infinity share the draw alone.  chances (may be null): w / sum of the token.
  * Weights are summed as integers, so that the draw does not depend on the order of summation: each is rounded to a multiple of 2^-k of the

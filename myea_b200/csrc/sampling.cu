@@ -596,7 +596,9 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
   d.from = min(d.first + d.warp * share, d.last);
   d.to = min(d.from + share, d.last);
   const float temperature = a.temperature == nullptr ? 1.f : a.temperature[row];
-  const float top_p = a.top_p == nullptr ? 1.f : a.top_p[row], min_p = a.min_p == nullptr ? 0.f : a.min_p[row], uniform = a.uniform[row];
+  const float top_p = a.top_p == nullptr ? 1.f : a.top_p[row], uniform = a.uniform[row];
+  float min_p = a.min_p == nullptr ? 0.f : a.min_p[row];
+  if (min_p > 1.f) min_p = 1.f;   // (the largest word's weight: it always stays)
   const int top_k = a.top_k == nullptr ? 0 : a.top_k[row];
 
   float m = -INFINITY;
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 4) sampling_kernel(const myea_sampli
   u64 least = 1;
   float reach = d.beyond;
   if (min_p > 0.f) {
-    least = min_p >= 1.f ? 1ull << shift : static_cast<u64>(ceil(ldexp(static_cast<double>(min_p), shift)));
+    least = static_cast<u64>(ceil(ldexp(static_cast<double>(min_p), shift)));
     reach = fminf(reach, -logf(min_p) * 1.0001f + 1e-3f);
   }
   const float nearest = fmaxf(m - reach * 1.001f * temperature, fmaxf(kept.value, -3.402823466e38f));
