@@ -27,6 +27,7 @@ namespace {
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kParts = 8, kList = 1024, kLongRow = 32;
+constexpr size_t kSharedMost = 200u << 10;   // bytes of a block
 static_assert(kThreads == 256, "a thread makes one entry of the table");
 constexpr double kLog2e64 = 1.4426950408889634074, kLn2 = 0.69314718055994530942;
 
@@ -710,7 +711,8 @@ int shift_for(uint64_t vocabulary) {
 }
 
 template <typename T, bool RES> cudaError_t launch(const myea_sampling &a, int parts, size_t smem, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(sampling_kernel<T, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // the most that any call takes, not this call's: the limit belongs to the function, whoever launches it
+  cudaError_t e = cudaFuncSetAttribute(sampling_kernel<T, RES>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSharedMost));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows * parts));
@@ -732,7 +734,7 @@ template <typename T> cudaError_t launch(const myea_sampling &a, cudaStream_t st
   int parts = 1;
   while (parts < kParts && (bytes / parts > (36u << 10) || (a.rows * parts * 2 <= 2 * kSms && a.vocabulary / (parts * 2) >= 4096))) parts *= 2;
   const size_t slice = (bytes / parts + 64) / 16 * 16;
-  if (sizeof(Shared) + slice > (200u << 10) || slice / sizeof(T) > 65536) return launch<T, false>(a, parts, sizeof(Shared), stream);
+  if (sizeof(Shared) + slice > kSharedMost || slice / sizeof(T) > 65536) return launch<T, false>(a, parts, sizeof(Shared), stream);
   return launch<T, true>(a, parts, sizeof(Shared) + slice, stream);
 }
 

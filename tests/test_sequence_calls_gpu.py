@@ -1,8 +1,12 @@
 """Calls that the documentation of the sequence operators allows and that their other tests do not make."""
+import ctypes as C
 import math
+import threading
 
 import pytest
 import torch
+
+from myea_b200 import capi
 
 from test_sequence_gpu import DEV
 from test_sequence_outputs_gpu import check_sampling
@@ -27,3 +31,31 @@ def test_a_least_share_above_one_keeps_the_largest(v):
             check_sampling(y, u, min_p=min_p)
             check_sampling(y, u, torch.full((4,), 0.7, device=DEV), top_k, top_p, min_p)
             check_sampling(y, u, torch.full((4,), 1e30, device=DEV), None, top_p, min_p)
+
+
+def test_draws_from_several_host_threads():
+    """threads whose launches take different amounts of shared memory, each a tight loop of calls (a refused one is counted, not lost)"""
+    lib, rounds, sizes = capi.load(), 6000, (50, 32000, 1000, 60001)
+    gen = torch.Generator(device=DEV).manual_seed(70)
+    rows = [(torch.randn(1, v, generator=gen, device=DEV) * 2, torch.rand(1, generator=gen, device=DEV)) for v in sizes]
+    want = [check_sampling(x, u) for x, u in rows]
+    tokens = [torch.full_like(w, -7) for w in want]
+    streams = [torch.cuda.Stream() for _ in sizes]
+    torch.cuda.synchronize()
+    begin, refused = threading.Barrier(len(sizes)), [None] * len(sizes)
+
+    def draw(k):
+        (x, u), message = rows[k], C.create_string_buffer(256)
+        s = capi.Sampling(capi.TYPE_F32, 0, 1, sizes[k], logits=x.data_ptr(), logits_stride=sizes[k], uniform=u.data_ptr(), tokens=tokens[k].data_ptr())
+        begin.wait(60)
+        refused[k] = sum(lib.myea_b200_sample(0, C.byref(s), streams[k].cuda_stream, message, 256) != 0 for _ in range(rounds))
+
+    threads = [threading.Thread(target=draw, args=(k,)) for k in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert refused == [0] * len(sizes)
+    for a, b in zip(tokens, want):
+        assert torch.equal(a, b)
