@@ -317,12 +317,13 @@ int myea_b200_compute_error_device(myea_handle h, uint64_t batch, const float *d
 /* No counterpart in the reference.  Instead of compute_error, for a softmax output layer and the cross entropy: the error against a
  * teacher's best logits (myea_distillation below) for the rows that compute_error would score, [T][batch] lists of `top` entries in DEVICE
  * memory on this handle's GPU: index and teacher [T][batch][top], labels and weight [T][batch] (may be null).  Losses are
- * ACCUMULATED as by compute_error, `outputs` terms per row; accuracy is not scored.  Asynchronous on the handle's stream. */
+ * ACCUMULATED as by compute_error, `outputs` terms per row; accuracy is not scored.  Asynchronous on the handle's stream
+ * (myea_b200_stream): what writes the arrays before, or over them afterwards, has to be ordered with that stream. */
 int myea_b200_compute_error_distillation_device(myea_handle h, uint64_t batch, const int32_t *index, const float *teacher, uint64_t top,
                                                 const int32_t *labels, const float *weight, float temperature, float soft, float hard);
 /* No counterpart in the reference.  Draws one output of a softmax output layer for every row of the last forward pass (myea_sampling below),
  * [T][batch] values per array in DEVICE memory on this handle's GPU; settings and chances may be null.  Asynchronous on the
- * handle's stream. */
+ * handle's stream, in whose order the arrays are read and written. */
 int myea_b200_sample_outputs_device(myea_handle h, uint64_t batch, const float *uniform, const float *temperature, const int32_t *top_k,
                                     const float *top_p, const float *min_p, int32_t *tokens, float *chances);
 /* Reset__Loss (Data.hpp:823) / the accumulators behind Get__Loss (Data.hpp:2913). */

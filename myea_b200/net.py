@@ -4,6 +4,7 @@ compute_error, Backward_Pass -> backward, Update_Derivative_Weight -> update_der
 update_parameter); every method is a thin call into libmyea_b200.so and raises RuntimeError with the library's
 message when the status is not MYEA_OK.  There is no CPU path: without the library or without a GPU it raises.
 """
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -18,7 +19,7 @@ def _f32(a):
 class Net:
     def __init__(self, desc, opt=None, device=0):
         self.lib = capi.load()
-        self.desc, self.opt = desc, opt
+        self.desc, self.opt, self.device = desc, opt, device
         self.h = C.c_void_p()
         rc = self.lib.myea_b200_create(C.byref(self.h), C.byref(desc), device)
         if rc != 0:
@@ -36,7 +37,7 @@ class Net:
         """Neural_Network::Load (Neural_Network__Load.cpp:2323): the network the reference's `.nn` / `.net` files describe,
         built for `batch` rows with parameters and normalization averages uploaded; .opt holds the optimizer settings"""
         self = cls.__new__(cls)
-        self.lib = capi.load()
+        self.lib, self.device = capi.load(), device
         self.h = C.c_void_p()
         opt = capi.OptDesc()
         rc = self.lib.myea_b200_load(C.byref(self.h), str(path_dimension).encode(), str(path_general).encode(), int(batch), device, C.byref(opt))
@@ -170,25 +171,40 @@ class Net:
             raise ValueError("%s: expected a contiguous %s array %s on the GPU, got %s of %s on %s" % (name, dtype, shape, tuple(x.shape), x.dtype, x.device))
         return x.data_ptr()
 
+    @contextlib.contextmanager
+    def _in_order_with_torch(self):
+        """a call on torch tensors: the network's stream first waits for torch's current stream, which wrote them, and that one then for the
+        network's, so that what torch does next finds the results and may write over the arguments, or give their memory away"""
+        import torch
+        theirs = torch.cuda.current_stream(self.device)
+        ours = torch.cuda.ExternalStream(self.lib.myea_b200_stream(self.h), device=theirs.device)
+        ours.wait_stream(theirs)
+        try:
+            yield
+        finally:
+            theirs.wait_stream(ours)
+
     def compute_error_distillation(self, index, teacher, temperature=1.0, soft=1.0, hard=0.0, labels=None, weight=None):
         """instead of compute_error: the error against a teacher's best logits, index (int32) and teacher (float32) [T, batch, top], labels (int32) and
-        weight (float32) [T, batch] on the GPU; what wrote them has to be done (the call runs on the network's stream)"""
+        weight (float32) [T, batch] on the network's GPU; in order with torch's current stream, without waiting on the host"""
         rows = (self.T, getattr(self, "active_B", self.B))
         top = int(index.shape[-1])
-        self._ck(self.lib.myea_b200_compute_error_distillation_device(
-            self.h, rows[1], self._device_array("index", index, rows + (top,), "int32"), self._device_array("teacher", teacher, rows + (top,), "float32"), top,
-            self._device_array("labels", labels, rows, "int32"), self._device_array("weight", weight, rows, "float32"), temperature, soft, hard),
-            "compute_error_distillation")
+        at = self._device_array
+        arrays = (at("index", index, rows + (top,), "int32"), at("teacher", teacher, rows + (top,), "float32"), top, at("labels", labels, rows, "int32"),
+                  at("weight", weight, rows, "float32"))
+        with self._in_order_with_torch():
+            self._ck(self.lib.myea_b200_compute_error_distillation_device(self.h, rows[1], *arrays, temperature, soft, hard), "compute_error_distillation")
 
     def sample_outputs(self, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, chances=None):
         """draws one output for every row of the last forward pass into tokens (int32 [T, batch]), from uniform (float32 [T, batch] in [0, 1)) and
-        settings of that shape or None, all on the GPU; runs on the network's stream"""
+        settings of that shape or None, all on the network's GPU; in order with torch's current stream, without waiting on the host"""
         rows = (self.T, getattr(self, "active_B", self.B))
         at = self._device_array
-        self._ck(self.lib.myea_b200_sample_outputs_device(
-            self.h, rows[1], at("uniform", uniform, rows, "float32"), at("temperature", temperature, rows, "float32"), at("top_k", top_k, rows, "int32"),
-            at("top_p", top_p, rows, "float32"), at("min_p", min_p, rows, "float32"), at("tokens", tokens, rows, "int32"), at("chances", chances, rows, "float32")),
-            "sample_outputs")
+        arrays = (at("uniform", uniform, rows, "float32"), at("temperature", temperature, rows, "float32"), at("top_k", top_k, rows, "int32"),
+                  at("top_p", top_p, rows, "float32"), at("min_p", min_p, rows, "float32"), at("tokens", tokens, rows, "int32"),
+                  at("chances", chances, rows, "float32"))
+        with self._in_order_with_torch():
+            self._ck(self.lib.myea_b200_sample_outputs_device(self.h, rows[1], *arrays), "sample_outputs")
 
     def backward(self):
         self._ck(self.lib.myea_b200_backward(self.h, getattr(self, "active_B", self.B)), "backward")

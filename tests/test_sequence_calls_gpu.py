@@ -3,12 +3,15 @@ import ctypes as C
 import math
 import threading
 
+import numpy as np
 import pytest
 import torch
 
 from myea_b200 import capi
+from myea_b200.net import Net
 
 from test_sequence_gpu import DEV
+from test_sequence_net_gpu import network, parameters
 from test_sequence_outputs_gpu import check_sampling
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +62,55 @@ def test_draws_from_several_host_threads():
     assert refused == [0] * len(sizes)
     for a, b in zip(tokens, want):
         assert torch.equal(a, b)
+
+
+def busy():
+    """some 10 ms of work on the current stream"""
+    a = torch.ones(4096, 4096, device=DEV, dtype=torch.bfloat16)
+    for _ in range(100):
+        a = a @ a * 0.0
+    return a.sum().float()
+
+
+def test_network_calls_keep_the_order_of_torchs_stream():
+    """arguments that torch is still writing, that are written over or dropped behind the call, and results that torch reads next: no
+    synchronization in between"""
+    T, B, V = 3, 6, 21
+    net = Net(network(T, B, outputs=V, softmax=True), capi.opt(capi.OPT_GD, gd_lr=0.0))
+    net.set(capi.BUF_PARAMETERS, parameters(net, 3, 2))
+    net.forward(np.random.default_rng(2).standard_normal((T, B, 7)).astype(np.float32))
+    gen = torch.Generator(device=DEV).manual_seed(72)
+    index = torch.randint(V, (T, B, 5), generator=gen, device=DEV, dtype=torch.int32)
+    teacher, weight = torch.randn(T, B, 5, generator=gen, device=DEV), torch.rand(T, B, generator=gen, device=DEV)
+    uniform, top_p = torch.rand(T, B, generator=gen, device=DEV), torch.rand(T, B, generator=gen, device=DEV) * 0.9 + 0.05
+    busy()
+    torch.cuda.synchronize()
+    net.compute_error_distillation(index, teacher, weight=weight)
+    errors = net.errors(3)
+    tokens, chances = torch.full((T, B), -7, dtype=torch.int32, device=DEV), torch.zeros(T, B, device=DEV)
+    net.sample_outputs(uniform, tokens, top_p=top_p, chances=chances)
+    net.synchronize()
+    torch.cuda.synchronize()
+    assert (tokens >= 0).all() and np.abs(errors).max() > 0
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            late = [torch.zeros_like(v) for v in (index, teacher, weight)]
+            torch.cuda.synchronize()
+            late[2] += busy()
+            for to, v in zip(late, (index, teacher, weight)):
+                to += v
+            net.compute_error_distillation(late[0], late[1], weight=late[2])
+            for to in late:
+                to.zero_()
+            net.synchronize()
+            assert np.array_equal(net.errors(3), errors)
+            given, drawn, had = torch.zeros_like(uniform), torch.full_like(tokens, -7), torch.zeros_like(chances)
+            torch.cuda.synchronize()
+            given += busy()
+            given += uniform
+            net.sample_outputs(given, drawn, top_p=top_p * 1.0, chances=had)
+            given.fill_(0.999)
+            seen, share = drawn.clone(), had.clone()   # (torch reads behind the network's kernel)
+            assert torch.equal(seen, tokens) and torch.equal(share, chances)
+            torch.cuda.synchronize()
+    net.close()
