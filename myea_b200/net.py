@@ -167,8 +167,9 @@ class Net:
         """address of an array on this network's GPU (a torch tensor); None where there is none"""
         if x is None:
             return None
-        if tuple(x.shape) != shape or not str(x.dtype).endswith(dtype) or not x.is_cuda or not x.is_contiguous():
-            raise ValueError("%s: expected a contiguous %s array %s on the GPU, got %s of %s on %s" % (name, dtype, shape, tuple(x.shape), x.dtype, x.device))
+        if tuple(x.shape) != shape or not str(x.dtype).endswith(dtype) or not x.is_cuda or x.get_device() != self.device or not x.is_contiguous():
+            raise ValueError("%s: expected a contiguous %s array %s on cuda:%d, got %s of %s on %s" % (name, dtype, shape, self.device, tuple(x.shape), x.dtype,
+                                                                                                       x.device))
         return x.data_ptr()
 
     @contextlib.contextmanager

@@ -1,0 +1,29 @@
+"""Calls of the sequence operators that are refused before a GPU is touched, beside those of their other tests."""
+import pytest
+import torch
+
+from myea_b200.net import Net
+
+
+class OnGpu:
+    """what a network asks of a tensor, as if it lay on a GPU"""
+    def __init__(self, index, shape=(2, 3), dtype=torch.float32, dense=True):
+        self.index, self.shape, self.dtype, self.device, self.is_cuda, self.dense = index, torch.Size(shape), dtype, torch.device("cuda", index), True, dense
+
+    def get_device(self):
+        return self.index
+
+    def is_contiguous(self):
+        return self.dense
+
+    def data_ptr(self):
+        return 4096
+
+
+def test_a_network_takes_arrays_of_its_own_gpu():
+    net = Net.__new__(Net)   # (without a handle: a GPU has to be there for one)
+    net.h, net.device = None, 1
+    assert net._device_array("weight", OnGpu(1), (2, 3), "float32") == 4096 and net._device_array("weight", None, (2, 3), "float32") is None
+    for other in (OnGpu(0), OnGpu(1, (3, 2)), OnGpu(1, dtype=torch.int32), OnGpu(1, dense=False), torch.zeros(2, 3)):
+        with pytest.raises(ValueError, match="cuda:1"):
+            net._device_array("weight", other, (2, 3), "float32")
