@@ -286,7 +286,9 @@ const char *check(const myea_scan *s, bool backward) {
   if (s->states < 1 || s->states > 128) return "selective_scan: 1 to 128 states";
   if (s->batch > kSequenceMost || s->time > kSequenceMost || s->width > kSequenceMost) return "selective_scan: a dimension above 2^30";
   if (s->groups < 1 || (s->width % s->groups) != 0) return "selective_scan: the groups have to divide the width";
-  if (s->batch == 0 || s->width == 0) return nullptr;
+  if (s->width == 0) return nullptr;
+  if (backward && s->d_A == nullptr) return "selective_scan: no array for the derivatives of A";   // (written as 0 for no sequences)
+  if (s->batch == 0) return nullptr;
   if (s->A == nullptr) return "selective_scan: no decay rates (A)";
   if (s->time > 0 && (s->u.data == nullptr || s->delta.data == nullptr || s->B.data == nullptr || s->C.data == nullptr)) return "selective_scan: u, delta, B or C is missing";
   if (s->checkpoints != nullptr && !aligned(s->checkpoints, 16)) return "selective_scan: checkpoints that are not 16-byte aligned";
@@ -300,7 +302,6 @@ const char *check(const myea_scan *s, bool backward) {
     return "selective_scan: dy, du, ddelta, dB or dC is missing";
   if (s->time > 0 && (s->z.data != nullptr) != (s->dz.data != nullptr)) return "selective_scan: dz goes with z";
   if (s->time > 0 && s->checkpoints == nullptr) return "selective_scan: the backward pass needs the forward pass's checkpoints";
-  if (s->d_A == nullptr) return "selective_scan: no array for the derivatives of A";
   if (s->d_state != nullptr && s->d_state == s->d_final_state) return "selective_scan: d_state may not be d_final_state";
   return nullptr;
 }

@@ -4,6 +4,8 @@ import torch
 
 from myea_b200.net import Net
 
+from test_sequence_cpu import ADDRESS, refused, scan
+
 
 class OnGpu:
     """what a network asks of a tensor, as if it lay on a GPU"""
@@ -27,3 +29,9 @@ def test_a_network_takes_arrays_of_its_own_gpu():
     for other in (OnGpu(0), OnGpu(1, (3, 2)), OnGpu(1, dtype=torch.int32), OnGpu(1, dense=False), torch.zeros(2, 3)):
         with pytest.raises(ValueError, match="cuda:1"):
             net._device_array("weight", other, (2, 3), "float32")
+
+
+def test_a_scan_over_no_sequences_needs_its_derivative_arrays():
+    """the derivatives of A are written (as 0) for an empty batch too"""
+    assert "derivatives of A" in refused("selective_scan_backward", scan(batch=0, d_A=None), None, 0)
+    assert "derivatives of A" in refused("selective_scan_backward", scan(batch=0, time=0, d_A=None, d_D=ADDRESS), None, 0)
