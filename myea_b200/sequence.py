@@ -4,7 +4,8 @@ formulas stand).  They stand beside the recurrent layers, the output error and t
 Tensors are torch tensors, used where they lie: an activation is [batch, time, width] with any strides over batch and time
 and densely packed last dimensions (a time-major array is x.transpose(0, 1), a slice of a wider projection is read in place),
 of float32, bfloat16 or float16, one type per call; parameters, states of a scan and losses are float32.  A call runs on the
-current stream of the tensors' GPU, may be captured into a CUDA graph and does not wait.  ValueError: the arguments do not fit
+current stream of the tensors' GPU, may be captured into a CUDA graph and does not wait.  Autograd does not follow it: derivatives come
+from the *_backward functions and the errors, and tensors that want a gradient are refused where gradients are recorded.  ValueError: the arguments do not fit
 together (nothing was launched); RuntimeError: the library refused the call or failed, with its message.
 """
 import ctypes as C
@@ -38,6 +39,10 @@ def _call(name, index, *args):
         raise RuntimeError("%s failed (%d): %s" % (name, rc, message.value.decode()))
 
 
+def _no_history(name):
+    raise ValueError("%s wants a gradient, which autograd would lose here: detach it or call under torch.no_grad(), and use the operator's derivatives" % name)
+
+
 def _mismatch(name, x, shape, dtype, index):
     raise ValueError("%s: expected %s of %s on cuda:%d, got %s of %s on %s" % (name, tuple(shape), dtype, index, tuple(x.shape), x.dtype, x.device))
 
@@ -66,6 +71,8 @@ def _view(name, x, shape, dtype, index):
         return _NO_VIEW
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
         _mismatch(name, x, shape, dtype, index)
+    if x.requires_grad and torch.is_grad_enabled():
+        _no_history(name)
     if not x.is_contiguous() and not _dense(x, 2):
         raise ValueError("%s: the dimensions behind batch and time have to lie densely, strides are %s" % (name, x.stride()))
     strides = x.stride()
@@ -78,6 +85,8 @@ def _array(name, x, shape, dtype, index):
         return 0
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
         _mismatch(name, x, shape, dtype, index)
+    if x.requires_grad and torch.is_grad_enabled():
+        _no_history(name)
     if not x.is_contiguous():
         raise ValueError("%s has to be contiguous" % name)
     return x.data_ptr()
@@ -221,12 +230,14 @@ def selective_scan_backward(dy, u, delta, A, B, C_, checkpoints, D=None, z=None,
     return got
 
 
-def _rows(name, x, shape, dtype, index):
-    """address and row pitch of a [rows, columns] tensor"""
+def _rows(name, x, shape, dtype, index, history=False):
+    """address and row pitch of a [rows, columns] tensor; history: autograd may follow it"""
     if x is None:
         return 0, 0
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
         _mismatch(name, x, shape, dtype, index)
+    if not history and x.requires_grad and torch.is_grad_enabled():
+        _no_history(name)
     if not x.is_contiguous() and not _dense(x, 1):
         raise ValueError("%s: the columns have to lie densely, strides are %s" % (name, x.stride()))
     return x.data_ptr(), x.stride(0)
@@ -257,7 +268,8 @@ def distillation_error(logits, index, teacher, temperature=1.0, soft=1.0, hard=0
 def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, chances=None):
     """(tokens int32 [rows], chances [rows]): one token for every row of logits [rows, vocabulary], drawn with uniform (float32 [rows], in
     [0, 1)) from what temperature, top_k (int32), top_p and min_p leave of the row, each an array of one value per row or None; and
-    the chance that it had.  temperature <= 0: the largest logit.  A row whose words are all closed (minus infinity): token -1."""
+    the chance that it had.  temperature <= 0: the largest logit.  A row whose words are all closed (minus infinity): token -1.  A draw
+    has no derivatives: the logits may want a gradient, the results have no history."""
     kind = _type(logits)
     if logits.dim() != 2:
         raise ValueError("logits is [rows, vocabulary]")
@@ -268,7 +280,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     if chances is None:
         chances = torch.empty_like(uniform) if uniform is not None else logits.new_empty(one, dtype=_F32)
     _call("myea_b200_sample", at, _SAMPLING.pack(
-        kind, 0, r, v, *_rows("logits", logits, (r, v), logits.dtype, at), _array("uniform", uniform, one, _F32, at), _array("temperature", temperature, one, _F32, at),
+        kind, 0, r, v, *_rows("logits", logits, (r, v), logits.dtype, at, True), _array("uniform", uniform, one, _F32, at), _array("temperature", temperature, one, _F32, at),
         _array("top_k", top_k, one, _I32, at), _array("top_p", top_p, one, _F32, at), _array("min_p", min_p, one, _F32, at),
         _array("tokens", tokens, one, _I32, at), _array("chances", chances, one, _F32, at)))
     return tokens, chances

@@ -7,10 +7,10 @@ import numpy as np
 import pytest
 import torch
 
-from myea_b200 import capi
+from myea_b200 import capi, sequence
 from myea_b200.net import Net
 
-from test_sequence_gpu import DEV
+from test_sequence_gpu import DEV, normal, scan_inputs
 from test_sequence_net_gpu import network, parameters
 from test_sequence_outputs_gpu import check_sampling
 
@@ -114,3 +114,29 @@ def test_network_calls_keep_the_order_of_torchs_stream():
             assert torch.equal(seen, tokens) and torch.equal(share, chances)
             torch.cuda.synchronize()
     net.close()
+
+
+def test_tensors_that_want_a_gradient_are_refused():
+    """autograd does not see these calls: rather an error than a result without history"""
+    i = scan_inputs(73, torch.float32, 1, 4, 8, 4, 1)
+    w = normal(torch.Generator(device=DEV).manual_seed(1), 8, 4)
+    logits, index, teacher = normal(torch.Generator(device=DEV).manual_seed(2), 2, 9), torch.zeros(2, 1, dtype=torch.int32, device=DEV), torch.zeros(2, 1, device=DEV)
+    scan = lambda j: sequence.selective_scan(j["u"], j["delta"], j["A"], j["B"], j["C"], D=j["D"], z=j["z"], delta_bias=j["bias"], state=j["state"])  # noqa: E731
+    wants = lambda v: v.clone().requires_grad_()  # noqa: E731
+    for name in ("u", "delta", "A", "B", "C", "D", "z", "bias", "state"):
+        with pytest.raises(ValueError, match="gradient"):
+            scan({**i, name: wants(i[name])})
+    for call in (lambda: sequence.causal_convolution(wants(i["u"]), w), lambda: sequence.causal_convolution(i["u"], wants(w)),
+                 lambda: sequence.causal_convolution(i["u"], w, out=wants(i["u"])), lambda: sequence.causal_convolution_backward(wants(i["dy"]), i["u"], w),
+                 lambda: sequence.distillation_error(wants(logits), index, teacher), lambda: sequence.distillation_error(logits, index, wants(teacher)),
+                 lambda: sequence.distillation_error(logits, index, teacher, weight=wants(teacher[:, 0]))):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():   # and where nothing is recorded they are like any other
+        for a, b in zip(scan({k: wants(v) for k, v in i.items()}), scan(i)):
+            assert torch.equal(a, b)
+        sequence.causal_convolution(i["u"], wants(w), out=torch.nn.Parameter(i["u"].clone()))
+        assert torch.equal(sequence.distillation_error(wants(logits), index, teacher)[1], sequence.distillation_error(logits, index, teacher)[1])
+    # a draw is whole numbers, which have no gradient anywhere
+    u = torch.tensor([0.3, 0.6], device=DEV)
+    assert torch.equal(sequence.sample(wants(logits), u)[0], sequence.sample(logits, u)[0])
