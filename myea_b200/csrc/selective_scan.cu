@@ -25,9 +25,7 @@ __global__ void __launch_bounds__(2 * S::NT) scan_forward_kernel(const ScanArgs 
     for (int q = 0; q < CPT; ++q) {
       const int have = p.have(a, q);
       const long long d = p.first + p.c + q;
-      const float4 a4 = parameters4(a.s.A + d * a.states + p.n, have);
-      A[q][0] = make_float2(a4.x * kLog2e, a4.y * kLog2e);
-      A[q][1] = make_float2(a4.z * kLog2e, a4.w * kLog2e);
+      rates2(parameters4(a.s.A + d * a.states + p.n, have), A[q]);
       float4 start = make_float4(0.f, 0.f, 0.f, 0.f);
       if (!STATES && have > 0) {
         if (a.chunks > 1) start = p.states_at(a.carry, p.b * a.chunks + p.chunk, a, q);
@@ -157,8 +155,8 @@ __global__ void __launch_bounds__(256, 3) scan_steps_kernel(const ScanArgs a, in
   const int first = group * a.per_group + in_group, channels = min(CH, a.per_group - in_group);
   const int have = c < channels ? min(4, a.states - n) : 0;
   const bool gate = a.s.z.data != nullptr;
-  const float4 a4 = load_states(a.s.A + static_cast<long long>(first + c) * a.states + n, have, a.vec_A);
-  const float2 A0 = make_float2(a4.x * kLog2e, a4.y * kLog2e), A1 = make_float2(a4.z * kLog2e, a4.w * kLog2e);
+  float2 A[2];
+  rates2(load_states(a.s.A + static_cast<long long>(first + c) * a.states + n, have, a.vec_A), A);
   for (int b0 = blockIdx.y * NB; b0 < a.batch; b0 += gridDim.y * NB) {
     float2 h[NB][2];
     const long long held = static_cast<long long>(a.width) * a.states, own = static_cast<long long>(first + c) * a.states + n;
@@ -209,8 +207,8 @@ __global__ void __launch_bounds__(256, 3) scan_steps_kernel(const ScanArgs a, in
       for (int k = 0; k < NB; ++k) {
         const float2 step = s_step[k * CH + c];
         const float4 b4 = at4(s_B + k * NP + n), c4 = at4(s_C + k * NP + n);
-        h[k][0] = fma2(decay2(both(step.x), A0), h[k][0], mul2(both(step.y), lo(b4)));
-        h[k][1] = fma2(decay2(both(step.x), A1), h[k][1], mul2(both(step.y), hi(b4)));
+        h[k][0] = fma2(decay2(both(step.x), A[0]), h[k][0], mul2(both(step.y), lo(b4)));
+        h[k][1] = fma2(decay2(both(step.x), A[1]), h[k][1], mul2(both(step.y), hi(b4)));
         const float2 r = fma2(h[k][1], hi(c4), mul2(h[k][0], lo(c4)));
         float y = r.x + r.y;
 #pragma unroll

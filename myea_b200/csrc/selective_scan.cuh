@@ -96,6 +96,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // 2^(s A).  The unit's results lie 2.0e-8 below 2^x on the average of x in -0.35 .. 0 (measured against 64 bits), the same way at every
 // step, which a state of long memory adds up: 2^-25 in the exponent takes that off.  (A step of length 0 still keeps the state.)
 __device__ __forceinline__ float2 decay2(float2 s, float2 A) { return exp2_fast(fma2(s, A, both(2.98023224e-8f))); }
+// A rate as a finite number (NaN stays), so that a step of length 0 has the product 0 and keeps the state whatever its rate
+__device__ __forceinline__ float finite_rate(float a) { return max_nan(a, -3.402823466e38f); }
+// the rates of four states, for decay2
+__device__ __forceinline__ void rates2(float4 a, float2 (&A)[2]) {
+  A[0] = make_float2(finite_rate(a.x * kLog2e), finite_rate(a.y * kLog2e));
+  A[1] = make_float2(finite_rate(a.z * kLog2e), finite_rate(a.w * kLog2e));
+}
 
 // log(1 + e^x) of two values, and its slope.  With e = e^-|x| <= 1 and q = e / (2 + e) <= 1/3:  log(1 + e) = 2 atanh(q) = 2 (q + q^3 / 3 +
 // ...), whose first term left out, q^15 / 15, is below 2^-26 of the sum.  The product |x| log2(e) is carried to 48 bits.
@@ -328,7 +335,8 @@ __global__ void __launch_bounds__(256) scan_chain_kernel(const ScanArgs a) {
   const long long row = id / LPC, b = row / a.width, d = row - b * a.width;
   if (b >= a.batch) return;
   const int have = min(4, a.states - n);
-  const float4 a4 = parameters4(a.s.A + d * a.states + n, have);
+  float4 a4 = parameters4(a.s.A + d * a.states + n, have);
+  a4 = make_float4(finite_rate(a4.x), finite_rate(a4.y), finite_rate(a4.z), finite_rate(a4.w));
   const float *start = BACKWARD ? a.s.d_final_state : a.s.state;
   float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
   if (start != nullptr) h = load_states(start + row * a.states + n, have, BACKWARD ? a.vec_d_final : a.vec_state);

@@ -83,9 +83,7 @@ __global__ void __launch_bounds__(S::NT) scan_backward_states_kernel(const ScanA
   float sum[CPT];
 #pragma unroll
   for (int q = 0; q < CPT; ++q) {
-    const float4 a4 = parameters4(a.s.A + static_cast<long long>(p.first + p.c + q) * a.states + p.n, p.have(a, q));
-    A[q][0] = make_float2(a4.x * kLog2e, a4.y * kLog2e);
-    A[q][1] = make_float2(a4.z * kLog2e, a4.w * kLog2e);
+    rates2(parameters4(a.s.A + static_cast<long long>(p.first + p.c + q) * a.states + p.n, p.have(a, q)), A[q]);
     g[q][0] = g[q][1] = both(0.f);
     sum[q] = 0.f;
   }
@@ -203,9 +201,7 @@ __global__ void __launch_bounds__(2 * S::NT, S::LPC <= 2 ? 1 : 2) scan_backward_
     for (int q = 0; q < CPT; ++q) {
       const int have = p.have(a, q);
       const long long d = p.first + p.c + q;
-      const float4 a4 = parameters4(a.s.A + d * a.states + p.n, have);
-      A[q][0] = make_float2(a4.x * kLog2e, a4.y * kLog2e);
-      A[q][1] = make_float2(a4.z * kLog2e, a4.w * kLog2e);
+      rates2(parameters4(a.s.A + d * a.states + p.n, have), A[q]);
       float4 end = make_float4(0.f, 0.f, 0.f, 0.f);
       if (have > 0) {
         if (a.chunks > 1) end = p.states_at(a.carry, p.b * a.chunks + p.chunk, a, q);

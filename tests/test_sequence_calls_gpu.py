@@ -10,7 +10,7 @@ import torch
 from myea_b200 import capi, sequence
 from myea_b200.net import Net
 
-from test_sequence_gpu import DEV, normal, scan_inputs
+from test_sequence_gpu import DEV, close, normal, run_scan, scan_inputs, scan_reference
 from test_sequence_net_gpu import network, parameters
 from test_sequence_outputs_gpu import check_sampling
 
@@ -140,3 +140,27 @@ def test_tensors_that_want_a_gradient_are_refused():
     # a draw is whole numbers, which have no gradient anywhere
     u = torch.tensor([0.3, 0.6], device=DEV)
     assert torch.equal(sequence.sample(wants(logits), u)[0], sequence.sample(logits, u)[0])
+
+
+@pytest.mark.parametrize("t,d,n", [(1, 20, 16), (21, 20, 16), (37, 9, 5), (600, 20, 16)])
+def test_rates_of_minus_infinity_forget_and_leave_the_other_steps_alone(t, d, n):
+    """a rate of minus infinity (or one that becomes it in the change of base) drops the state at every step; where there is no step, behind
+    a sequence's end and in the rest of a tile, the state stays.  The reference has -1e30 in its place, whose decays are the same 0
+    and 1; the tolerance is the one of the other scan tests, with the exponents of the finite rates."""
+    i = scan_inputs(74, torch.float32, 3, t, d, n, 1)
+    lengths = torch.tensor([t, t // 3, 0], dtype=torch.int32, device=DEV)
+    behind = torch.arange(t, device=DEV)[None] >= lengths[:, None]
+    for name in ("u", "delta", "B", "C", "z", "dy"):
+        i[name][behind] = math.nan
+    i["A"][::3, 1::2] = -math.inf
+    i["A"][1::3, 0] = torch.finfo(torch.float32).min
+    got = run_scan(i, True, lengths)
+    clean = {k: torch.nan_to_num(v.double()) for k, v in i.items()}
+    clean["A"] = i["A"].double().clamp(min=-1e30)
+    want, big = scan_reference(clean, True, lengths, False), scan_reference(clean, True, lengths, True)
+    exponents = scan_reference({**clean, "A": torch.where(clean["A"] < -1e20, -1.0, clean["A"])}, True, lengths, False)["exponents"]
+    once = (t + 16) * 2.0 ** -22 + (exponents + 4) * 2.0 ** -21 + 80 * 2.0 ** -23 + n * 2.0 ** -24
+    for name in want:
+        if name != "exponents":
+            sums = {"A": 3 * t, "D": 3 * t, "delta_bias": 3 * t, "B": d, "C": d}.get(name, 0)
+            close(name, got[name], want[name], (once + sums * 2.0 ** -24) * big[name])
