@@ -132,21 +132,19 @@ int scan_layer_create(myea_b200_net *net, LayerPlan &L) {
   if (rc == MYEA_OK) rc = device_array(net, &S->rates, S->D * S->N);
   if (rc == MYEA_OK) rc = device_array(net, &S->grads, S->count);
   if (rc != MYEA_OK) return rc;
-  // the most working memory that a batch of 1 .. B rows takes: fewer rows may cut the time into more chunks
-  const long long was = net->active_B;
-  for (long long b = net->full_pitch ? net->B : 1; b <= net->B; ++b) {
-    net->active_B = b;
+  // Working memory: shorter batches take no more.  With several time steps the arrays keep the rows of the longest batch, and a single
+  // step is never cut, so that its sizes go by the rows.
+  {
     myea_convolution c;
     myea_scan s;
     describe(net, L, &c, &s);
     // (addresses that stand for the backward pass's; only the sizes count here)
     c.d_weight = c.d_bias = s.d_A = S->grads;
-    c.dy = c.y; c.dx = rows_of(S->du, S->D, b);
+    c.dy = c.y; c.dx = rows_of(S->du, S->D, net->B);
     s.checkpoints = S->du; s.dy = s.y; s.du = s.ddelta = s.dB = s.dC = s.dz = c.dx;
-    S->work_bytes = std::max({S->work_bytes, myea_b200_selective_scan_workspace(&s), myea_b200_selective_scan_backward_workspace(&s),
+    S->work_bytes = std::max({myea_b200_selective_scan_workspace(&s), myea_b200_selective_scan_backward_workspace(&s),
                               myea_b200_causal_convolution_backward_workspace(&c)});
   }
-  net->active_B = was;
   myea_scan s = {};
   s.batch = static_cast<uint64_t>(net->B); s.time = static_cast<uint64_t>(net->T); s.width = static_cast<uint64_t>(S->D); s.states = static_cast<uint64_t>(S->N);
   rc = device_array(net, &S->checkpoints, myea_b200_selective_scan_checkpoint_bytes(&s) / sizeof(float));

@@ -1,10 +1,13 @@
 """Calls of the sequence operators that are refused before a GPU is touched, beside those of their other tests."""
+import ctypes as C
+
 import pytest
 import torch
 
+from myea_b200 import capi
 from myea_b200.net import Net
 
-from test_sequence_cpu import ADDRESS, refused, scan
+from test_sequence_cpu import ADDRESS, convolution, refused, scan
 
 
 class OnGpu:
@@ -35,3 +38,15 @@ def test_a_scan_over_no_sequences_needs_its_derivative_arrays():
     """the derivatives of A are written (as 0) for an empty batch too"""
     assert "derivatives of A" in refused("selective_scan_backward", scan(batch=0, d_A=None), None, 0)
     assert "derivatives of A" in refused("selective_scan_backward", scan(batch=0, time=0, d_A=None, d_D=ADDRESS), None, 0)
+
+
+@pytest.mark.parametrize("d,n,taps", [(1, 1, 1), (12, 5, 4), (64, 16, 4), (65, 128, 8)])
+def test_single_steps_of_fewer_rows_take_no_more_working_memory(d, n, taps):
+    """a network makes room for its whole batch and runs shorter ones"""
+    lib, before = capi.load(), (0, 0, 0)
+    for rows in list(range(1, 70)) + [148, 149, 296, 591, 592, 593, 1000, 4096, 65536]:
+        s, c = scan(batch=rows, time=1, width=d, states=n), convolution(batch=rows, time=1, width=d, taps=taps)
+        now = (lib.myea_b200_selective_scan_workspace(C.byref(s)), lib.myea_b200_selective_scan_backward_workspace(C.byref(s)),
+               lib.myea_b200_causal_convolution_backward_workspace(C.byref(c)))
+        assert now[1] > 0 and now[2] > 0 and all(a <= b for a, b in zip(before, now)), rows
+        before = now
