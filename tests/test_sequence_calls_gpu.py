@@ -11,8 +11,8 @@ from myea_b200 import capi, sequence
 from myea_b200.net import Net
 
 from test_sequence_gpu import DEV, close, normal, run_scan, scan_inputs, scan_reference
-from test_sequence_net_gpu import network, parameters
-from test_sequence_outputs_gpu import check_sampling
+from test_sequence_net_gpu import near, network, parameters, scan_layer, scan_parameters
+from test_sequence_outputs_gpu import check_sampling, distillation_reference, teacher_for
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +164,108 @@ def test_rates_of_minus_infinity_forget_and_leave_the_other_steps_alone(t, d, n)
         if name != "exponents":
             sums = {"A": 3 * t, "D": 3 * t, "delta_bias": 3 * t, "B": d, "C": d}.get(name, 0)
             close(name, got[name], want[name], (once + sums * 2.0 ** -24) * big[name])
+
+
+@pytest.mark.parametrize("dtype,r,v,tau,hard", [(torch.float32, 2, 50001, 4.0, 0.25), (torch.bfloat16, 2, 131072, 1.0, 0.0), (torch.float32, 300, 131072, 2.0, 0.5),
+                                                (torch.bfloat16, 600, 60001, 1.0, 0.0), (torch.float16, 203, 32001, 1.5, 0.25), (torch.bfloat16, 1200, 8003, 1.5, 0.5)])
+def test_long_rows_of_the_distillation_lose_no_word(dtype, r, v, tau, hard):
+    """Sums as exact as they are made: a thread adds up at most v / 256 + 128 words (a block has 256 threads or more, or eight packs of 8 words each), lanes,
+    warps and blocks add 5 + 4 + 3 times: depth * 2^-24.  A thread's maximum rises at most once for each 2 packs of 4 words that it reads, every warp's
+    and block's three times more; a rise multiplies by an exponential, which is off by E = 2^-22 + 2^-23 (R / T + 2) as the words' own are.  On random
+    logits a thread's maximum rises about ln(v / 256) times, 8 at most here; 16 are allowed.  A sum, and with it a gradient, is good to (16 + 5) E +
+    depth * 2^-24, below 2^-13 here: a share of the row that got lost shows."""
+    gen = torch.Generator(device=DEV).manual_seed(v + r)
+    x = (torch.randn(r, v, generator=gen, device=DEV) * 0.5).to(dtype)
+    index, teacher = teacher_for(gen, r, v, 5)
+    labels = torch.randint(v, (r,), generator=gen, device=DEV, dtype=torch.int32)
+    losses, d = sequence.distillation_error(x, index, teacher, tau, 1.0 - hard, hard, labels)
+    some = torch.arange(0, r, max(1, r // 6), device=DEV)
+    want, grad, want_big, grad_big = distillation_reference(x[some], index[some], teacher[some], tau, 1.0 - hard, hard, labels[some], None)
+    reach = (x.double().max() - x.double().min()).item()
+    reach = max(reach, (teacher.max() - teacher.min()).item())
+    e = 2.0 ** -22 + 2.0 ** -23 * (reach / min(tau, 1.0) + 2)
+    share = 21 * e + (v / 256 + 140) * 2.0 ** -24
+    assert share < 2.0 ** -13
+    off = (losses[some].double().cpu() - want).abs() - (share * (want_big + 1.0) + 2.0 ** -24 * want.abs())
+    assert off.max() <= 0, off.max()
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).tiny * (2.0 ** -10 if dtype == torch.float16 else 1)
+    off = (d[some].double().cpu() - grad).abs() - (half * grad.abs() + (1 + half) * share * grad_big + tiny)
+    assert off.max() <= 0, off.max()
+
+
+def directions(net, X, Y, layers, out):
+    """derivatives of every layer against differences of the loss: outputs good to 1e-6 of 1, a difference of losses of some 50 good to 2e-3 of its slope, and
+    the third derivative adds h^2"""
+    p = net.get(capi.BUF_PARAMETERS)
+    rng = np.random.default_rng(5)
+
+    def loss(params):
+        net.set(capi.BUF_PARAMETERS, params)
+        net.forward(X)
+        return 0.5 * float(((net.outputs(out).astype(np.float64) - Y) ** 2).sum())
+
+    net.forward(X)
+    net.compute_error(Y)
+    net.backward()
+    net.update_derivative_weight()
+    g = net.get(capi.BUF_DERIVATIVES).astype(np.float64)
+    for l in layers:
+        li = net.layer_index(l)
+        a, b = int(li.first_connection_index), int(li.last_connection_index)
+        way = np.zeros(net.P)
+        way[a:b] = rng.standard_normal(b - a)
+        way /= np.linalg.norm(way)
+        h = 1e-2
+        slope = (loss((p + h * way).astype(np.float32)) - loss((p - h * way).astype(np.float32))) / (2 * h)
+        assert abs(slope - g @ way) <= 1e-2 * np.linalg.norm(g[a:b]) + 1e-2, (l, slope, g @ way)
+    net.set(capi.BUF_PARAMETERS, p)
+
+
+@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("kind", ["normalized", "recurrent below", "lstm above", "pooling above", "recurrent above", "pooling below"])
+def test_scan_layer_among_layers_of_other_kinds(kind, T):
+    B, d, n = 6, 8, 4
+    wide = capi.selective_scan_inputs(d, n)
+    below = {"normalized": [capi.fc(wide, capi.AF_TANH, norm=capi.NORM_BN)], "recurrent below": [capi.fc_ind_rnn(wide, capi.AF_TANH)],
+             "pooling below": [capi.fc(wide, capi.AF_TANH), capi.pooling(capi.LAYER_AVERAGE_POOLING, 3, 1), capi.fc(wide, capi.AF_LINEAR)]}.get(kind, [capi.fc(wide, capi.AF_TANH)])
+    above = {"lstm above": [capi.lstm(3)], "pooling above": [capi.pooling(capi.LAYER_AVERAGE_POOLING, 2, 2)],
+             "recurrent above": [capi.fc_ind_rnn(7, capi.AF_TANH)]}.get(kind, [])
+    layers = [capi.fc(4)] + below + [capi.selective_scan(d, n, 3)] + above + [capi.fc(3, capi.AF_LINEAR)]
+    net = Net(capi.net(layers, B, T=T), capi.opt(capi.OPT_GD, gd_lr=0.0))
+    rng = np.random.default_rng(6)
+    p = (rng.standard_normal(net.P) * 0.3).astype(np.float32)
+    if net.n_norm:
+        p[net.W + net.n_bias:net.W + net.n_bias + net.n_norm] = 1.0
+    net.set(capi.BUF_PARAMETERS, p)
+    X, Y = rng.standard_normal((T, B, 4)).astype(np.float32), rng.standard_normal((T, B, 3)).astype(np.float32)
+    directions(net, X, Y, [l for l in range(1, len(layers)) if layers[l].type_layer not in (capi.LAYER_AVERAGE_POOLING,)], len(layers) - 1)
+    net.close()
+
+
+def test_scan_layer_behind_dropout():
+    """the scan reads the outputs that dropout leaves, and its error goes on to the layer below as for any other layer above it"""
+    T, B, d, n, k = 5, 4, 12, 5, 4
+    layers = [capi.fc(7), capi.fc(capi.selective_scan_inputs(d, n), capi.AF_TANH, dropout=capi.DROP_BERNOULLI, p=(0.7, 0.0, 0.0)), capi.selective_scan(d, n, k),
+              capi.fc(9, capi.AF_LINEAR)]
+    net = Net(capi.net(layers, B, T=T), capi.opt(capi.OPT_GD, gd_lr=0.0))
+    p = parameters(net, 9, 2, d, n, k)
+    net.set(capi.BUF_PARAMETERS, p)
+    rng = np.random.default_rng(7)
+    mask = (rng.random((T, capi.selective_scan_inputs(d, n))) < 0.7).astype(np.uint8)
+    net.set_mask_bernoulli(1, mask)
+    net.forward(rng.standard_normal((T, B, 7)).astype(np.float32))
+    net.compute_error(rng.standard_normal((T, B, 9)).astype(np.float32))
+    net.backward()
+    net.update_derivative_weight()
+    read = net.outputs(1)
+    assert (read[np.broadcast_to(mask[:, None] == 0, read.shape)] == 0).all() and (read != 0).any()
+    x, q = torch.tensor(read.astype(np.float64), requires_grad=True), torch.tensor(p.astype(np.float64), requires_grad=True)
+    y = scan_layer(x, scan_parameters(net, q, 2, d, n, k))
+    near(net.outputs(2), y, "outputs")
+    (y * torch.tensor(net.errors(2).astype(np.float64))).sum().backward()
+    near(net.errors(1), x.grad * (1 - x.detach() ** 2), "error below")   # (tanh's slope from its output)
+    li = net.layer_index(2)
+    a, b = int(li.first_connection_index), int(li.last_connection_index)
+    near(net.get(capi.BUF_DERIVATIVES)[a:b], q.grad[a:b], "derivatives")
+    net.close()
