@@ -304,6 +304,8 @@ const char *check(const myea_distillation *d) {
   return nullptr;
 }
 
+bool two_temperatures(const myea_distillation &d) { return d.hard != 0.f && d.temperature != 1.f && d.labels != nullptr; }
+
 template <typename T, int P> cudaError_t launch(const myea_distillation &d, int threads, int parts, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(d.rows * parts));
@@ -315,16 +317,20 @@ template <typename T, int P> cudaError_t launch(const myea_distillation &d, int 
   attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 1 : 0;
-  const bool two = d.hard != 0.f && d.temperature != 1.f && d.labels != nullptr;
-  return two ? cudaLaunchKernelEx(&cfg, distillation_kernel<T, true, P>, d) : cudaLaunchKernelEx(&cfg, distillation_kernel<T, false, P>, d);
+  return two_temperatures(d) ? cudaLaunchKernelEx(&cfg, distillation_kernel<T, true, P>, d) : cudaLaunchKernelEx(&cfg, distillation_kernel<T, false, P>, d);
 }
 
 template <typename T> cudaError_t launch(const myea_distillation &d, cudaStream_t stream) {
   const uint64_t packs = (d.vocabulary * sizeof(T) + 15) / 16;
   int parts = 1;
+  // Blocks that fill one SM and leave the next with half the work are halved where a block's exponentials outweigh the exchange between two:
+  // with 8 words in a pack and two temperatures (us, whole / halved: 203 rows of 16801, 25601, 32001 fp16 words 12.4 / 12.5, 15.4 / 14.5, 17.5 /
+  // 15.7; of as many packs in fp32 10.9 / 11.2, 12.2 / 12.6, 13.2 / 13.7, and in fp16 at one temperature 10.5 / 11.0, 12.1 / 12.5, 13.1 /
+  // 13.4), and in rows that are in blocks already (111 rows of 64001 fp16 words 19.1 / 17.7, at one temperature 14.3 / 14.1, of as many packs in
+  // fp32 14.6 / 14.3; 75 rows 17.9 / 15.1, 13.6 / 12.5, 13.8 / 12.7).
+  const bool heavy = sizeof(T) == 2 && two_temperatures(d);
   while (parts < 8 && ((d.rows * parts * 2 <= 2ull * kSms && packs >= parts * 2 * 256) ||
-                       // rows that fill one SM and leave the next with half the work (203 of 32001 fp16 logits: 16.4 us as they are, 14.5 in two)
-                       (d.rows * parts * 2 <= 3ull * kSms && packs > parts * 2048 && packs <= parts * 4096)))
+                       (d.rows * parts * 2 <= 3ull * kSms && packs > parts * 2048 && packs <= parts * 4096 && (parts > 1 || heavy))))
     parts *= 2;
   const uint64_t share = (packs + parts - 1) / parts;
   // Many rows: few threads with eight packs each, so that more rows lie side by side and the join of a row's warps is short (2000 rows of

@@ -167,7 +167,8 @@ def test_rates_of_minus_infinity_forget_and_leave_the_other_steps_alone(t, d, n)
 
 
 @pytest.mark.parametrize("dtype,r,v,tau,hard", [(torch.float32, 2, 50001, 4.0, 0.25), (torch.bfloat16, 2, 131072, 1.0, 0.0), (torch.float32, 300, 131072, 2.0, 0.5),
-                                                (torch.bfloat16, 600, 60001, 1.0, 0.0), (torch.float16, 203, 32001, 1.5, 0.25), (torch.bfloat16, 1200, 8003, 1.5, 0.5)])
+                                                (torch.bfloat16, 600, 60001, 1.0, 0.0), (torch.float16, 203, 32001, 1.5, 0.25), (torch.bfloat16, 1200, 8003, 1.5, 0.5),
+                                                (torch.float32, 203, 16001, 1.5, 0.25), (torch.bfloat16, 203, 32001, 1.0, 0.0), (torch.float16, 111, 64001, 2.0, 0.5)])
 def test_long_rows_of_the_distillation_lose_no_word(dtype, r, v, tau, hard):
     """Sums as exact as they are made: a thread adds up at most v / 256 + 128 words (a block has 256 threads or more, or eight packs of 8 words each), lanes,
     warps and blocks add 5 + 4 + 3 times: depth * 2^-24.  A thread's maximum rises at most once for each 2 packs of 4 words that it reads, every warp's
