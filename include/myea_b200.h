@@ -474,8 +474,8 @@ int myea_b200_selective_scan_backward(int device, const myea_scan *s, void *work
  * the row's teacher logits over temperature, q the softmax of `logits` over temperature and r the softmax of `logits`:
  *   losses[row] = weight[row] * (soft * temperature^2 * sum over entries of p * (log p - log q[index]) - hard * log r[label])
  * d_logits (null: only the losses; may be `logits`): the derivatives of losses[row] with respect to the row's logits, of their type.  A
- * row without entries has no soft term, a label outside the vocabulary (or labels = null) no hard term, and a row of weight 0 is not
- * read: loss and derivatives are 0.  Logits of minus infinity are closed words; a row without an open one has no softmax and counts
+ * row without entries has no soft term, a label outside the vocabulary (or labels = null) no hard term, and of a row of weight 0 nothing
+ * counts, not even NaN: loss and derivatives are 0.  Logits of minus infinity are closed words; a row without an open one has no softmax and counts
  * as one of weight 0.  Rows are stride elements apart.  1 <= top <= 1024,
  * temperature > 0. */
 typedef struct myea_distillation {

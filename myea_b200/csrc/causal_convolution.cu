@@ -4,7 +4,9 @@
 // Bound by memory: a handful of multiply-adds per element.  A thread takes four channels (8 or 16 bytes) over a run of
 // positions and keeps the last W inputs, and backward the W errors that are not complete yet, in registers, so each element is
 // read from memory once; the W - 1 positions that neighbouring runs share come out of L2.  What holds it back is the number of warps
-// that fit beside such registers: 4 x 2048 x 4096 bf16 with 4 taps take 40 us forward (3.4 TB/s) and 73 us backward (2.8 TB/s).
+// that fit beside such registers: a thread's loads, arithmetic and stores take turns, and few others fill in.  4 x 2048 x 4096 bf16
+// with 4 taps take 40 us forward (3.4 TB/s) and 73 us backward (2.8 TB/s), in fp32 58 and 128 (4.7 and 3.1 TB/s; backward
+// 64 words of a thread go through local memory).
 // Measured with shorter runs: two blocks per SM instead of three 52 us for 48, backward one instead of two 122 us for 81.  Loads
 // eight positions ahead instead of four 38 us, but 4.4 us in place of 3.7 for single positions of 64 sequences.
 #include <math.h>
@@ -244,7 +246,8 @@ __global__ void __launch_bounds__(256) convolution_finish_kernel(const float *pa
 }
 
 // A run's positions: the launch takes as long as its waves of blocks, each as long as a run, the positions that a run reads twice and
-// what a thread does once (together some 8 positions).  4 x 2048 x 4096: 80 forward and 128 backward, one wave each.
+// what a thread does once (together some 8 positions).  4 x 2048 x 4096: 80 forward and 128 backward, one wave each.  (Above four taps one
+// block per SM is reckoned with; forward, up to six taps and with 16-bit types seven, two fit.)
 int run_length(const myea_convolution *c, bool backward) {
   const int64_t resident = kSms * (c->taps > 4 ? 1 : backward ? 2 : 3), batch = static_cast<int64_t>(c->batch), time = static_cast<int64_t>(c->time);
   const int64_t groups = (static_cast<int64_t>(c->width) + 3) / 4;

@@ -7,7 +7,7 @@
 // stay in registers from the one time that they are read until their gradient is written.  Longer ones are read twice, the second
 // time out of L2: 296 rows of 256 KB at a time fit there as long as the gradients, which nobody reads here, are stored past it
 // (stored the ordinary way a third of the second reading came out of memory again).  2048 rows of 131072 bf16 logits: 252 us, 4.3 TB/s
-// of 6.5; a block of 1024 threads per SM 272 us, registers of clusters of four 422 us, most of it waiting for one another.
+// of 6.5 (115 us for the losses alone; the second reading asks for its packs right before it uses them); a block of 1024 threads per SM 272 us, registers of clusters of four 422 us, most of it waiting for one another.
 // Many short rows are bound by a row's chain of steps, so as many blocks as can be lie side by side: 4096 rows of 1024 fp32 logits
 // 18.3 us with 40 registers a thread, 19.3 with 54, 20.8 as clusters of one block, 28 with a warp per row.
 // A cluster of blocks takes a row only where the rows leave SMs idle; the blocks' parts of the sums are exchanged through

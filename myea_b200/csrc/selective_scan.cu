@@ -8,7 +8,9 @@ namespace {
 // STATES: only the states at the chunks' ends from a zero start, and the sums of their step lengths.
 // One half of the block's warps walk over the steps of a tile while the other half make the tile after it (step lengths, products)
 // and finish the one before it (skip, gate, stores): the two kinds of work have different dependencies, and a chip that is
-// not full of channels has twice the warps to hide them behind.
+// not full of channels has twice the warps to hide them behind.  What bounds it are the warps that walk: with 16 states and 16-bit types two blocks
+// fit on an SM, 8 such warps, and keep its unit for powers 61 % busy (4096 x 4096 channels in one sequence: 123 us, and 97 for STATES); fp32
+// inputs on their way take 166 registers a thread, one block per SM and 176 us.
 template <typename T, typename S, bool STATES>
 __global__ void __launch_bounds__(2 * S::NT) scan_forward_kernel(const ScanArgs a) {
   constexpr int CPT = S::CPT, PAIRS = S::PAIRS, BC = S::BC;
@@ -250,8 +252,9 @@ template <typename S> constexpr size_t forward_smem() { return (4 * S::PAIRS + 4
 
 template <typename T, typename S> cudaError_t launch_forward(const ScanArgs &a, cudaStream_t stream) {
   const long long blocks = static_cast<long long>(a.tiles) * a.groups * a.batch;
-  // Measured at 4096 channels of 16 states in bf16: 256 sequences of 1 / 4 positions 40 / 89 us against 215 / 219 staged, 16 of them 5.2 /
-  // 11.5 against 16; with a sequence per block, which a single one needs, 3.0 us against 4.0, but two positions 4.8.
+  // Measured at 4096 channels of 16 states in bf16: 256 sequences of 1 / 2 / 4 positions 40 / 57 / 88 us against 215 to 220 staged, whatever
+  // number up to 16 it is (a whole tile is walked, and a block with one tile has nothing to do beside it); 16 sequences 5.2 / - / 11.5 against 16;
+  // with a sequence per block, which a single one needs, 3.0 us against 4.0, but two positions 4.8.
   const bool many = blocks >= 4 * kSms;
   if (a.time <= (many ? 4 : 1)) {
     if (many) launch_steps<T, S::LPC, 8>(a, stream);
