@@ -179,6 +179,12 @@ class Net:
         import torch
         theirs = torch.cuda.current_stream(self.device)
         ours = torch.cuda.ExternalStream(self.lib.myea_b200_stream(self.h), device=theirs.device)
+        if theirs.cuda_stream == ours.cuda_stream:
+            yield
+            return
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a call of a network runs on the network's stream: a graph that is captured from another one would not order it behind the forward pass")
         ours.wait_stream(theirs)
         try:
             yield

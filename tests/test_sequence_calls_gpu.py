@@ -270,3 +270,29 @@ def test_scan_layer_behind_dropout():
     a, b = int(li.first_connection_index), int(li.last_connection_index)
     near(net.get(capi.BUF_DERIVATIVES)[a:b], q.grad[a:b], "derivatives")
     net.close()
+
+
+def test_network_calls_are_not_captured_from_another_stream():
+    """the network's forward pass runs on its own stream, whatever torch captures: replays would draw from whatever lies there"""
+    T, B, V = 2, 3, 9
+    net = Net(network(T, B, outputs=V, softmax=True), capi.opt(capi.OPT_GD, gd_lr=0.0))
+    net.set(capi.BUF_PARAMETERS, parameters(net, 4, 2))
+    net.forward(np.random.default_rng(3).standard_normal((T, B, 7)).astype(np.float32))
+    index, teacher = torch.zeros(T, B, 2, dtype=torch.int32, device=DEV), torch.zeros(T, B, 2, device=DEV)
+    uniform, tokens = torch.full((T, B), 0.4, device=DEV), torch.full((T, B), -7, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        uniform.mul_(1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            net.sample_outputs(uniform, tokens)
+        with pytest.raises(RuntimeError, match="captured"):
+            net.compute_error_distillation(index, teacher)
+    assert (tokens == -7).all()
+    with torch.cuda.stream(torch.cuda.ExternalStream(net.lib.myea_b200_stream(net.h))):   # torch on the network's own stream: in order anyway
+        net.sample_outputs(uniform, tokens)
+        seen = tokens.clone()
+    torch.cuda.synchronize()
+    assert ((seen >= 0) & (seen < V)).all()
+    net.compute_error_distillation(index, teacher)
+    net.synchronize()
+    net.close()
