@@ -71,12 +71,26 @@ def _view(name, x, shape, dtype, index):
         return _NO_VIEW
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
         _mismatch(name, x, shape, dtype, index)
+    return _own_view(name, x)
+
+
+def _own_view(name, x):
+    """the same for the tensor that the others are compared with"""
     if x.requires_grad and torch.is_grad_enabled():
         _no_history(name)
     if not x.is_contiguous() and not _dense(x, 2):
         raise ValueError("%s: the dimensions behind batch and time have to lie densely, strides are %s" % (name, x.stride()))
     strides = x.stride()
     return x.data_ptr(), strides[0], strides[1]
+
+
+def _output(name, given, like):
+    """(tensor, its address and strides): the given one, or a new one like `like`"""
+    if given is not None:
+        return given, _view(name, given, like.shape, like.dtype, like.get_device())
+    new = _empty_like(like)
+    _, t, d = like.shape
+    return new, (new.data_ptr(), t * d, d)
 
 
 def _array(name, x, shape, dtype, index):
@@ -122,13 +136,12 @@ def causal_convolution(x, weight, bias=None, silu=True, state=None, final_state=
     if x.dim() != 3 or weight.dim() != 2:
         raise ValueError("x is [batch, time, width] and weight [width, taps]")
     (b, t, d), k, tp, at = x.shape, weight.shape[1], x.dtype, x.get_device()
-    whole, before = (b, t, d), (b, k - 1, d)
-    if out is None:
-        out = _empty_like(x)
+    before = (b, k - 1, d)
+    out, to = _output("out", out, x)
     if final_state is None:
         final_state = x.new_empty(before)
     _call("myea_b200_causal_convolution", at, _CONVOLUTION.pack(
-        kind, k, 1 if silu else 0, 0, b, t, d, *_view("x", x, whole, tp, at), *_view("out", out, whole, tp, at), *_NO_VIEW, *_NO_VIEW,
+        kind, k, 1 if silu else 0, 0, b, t, d, *_own_view("x", x), *to, *_NO_VIEW, *_NO_VIEW,
         _array("weight", weight, (d, k), _F32, at), _array("bias", bias, (d,), _F32, at), _array("state", state, before, tp, at),
         _array("final_state", final_state, before, tp, at), _array("lengths", lengths, (b,), _I32, at), 0, 0, 0, 0))
     return out, final_state
@@ -143,14 +156,13 @@ def causal_convolution_backward(dy, x, weight, bias=None, silu=True, state=None,
         raise ValueError("x is [batch, time, width] and weight [width, taps]")
     (b, t, d), k, tp, at = x.shape, weight.shape[1], x.dtype, x.get_device()
     whole, before = (b, t, d), (b, k - 1, d)
-    if dx is None:
-        dx = _empty_like(x)
+    dx, to = _output("dx", dx, x)
     d_weight = _gradient("d_weight", d_weight, (d, k), x, accumulate)
     d_bias = _gradient("d_bias", d_bias, (d,), x, accumulate) if bias is not None else None
     d_state = x.new_empty(before) if state is not None else None
     s = _CONVOLUTION.pack(
-        kind, k, 1 if silu else 0, 1 if accumulate else 0, b, t, d, *_view("x", x, whole, tp, at), *_NO_VIEW, *_view("dy", dy, whole, tp, at),
-        *_view("dx", dx, whole, tp, at), _array("weight", weight, (d, k), _F32, at), _array("bias", bias, (d,), _F32, at), _array("state", state, before, tp, at),
+        kind, k, 1 if silu else 0, 1 if accumulate else 0, b, t, d, *_own_view("x", x), *_NO_VIEW, *_view("dy", dy, whole, tp, at),
+        *to, _array("weight", weight, (d, k), _F32, at), _array("bias", bias, (d,), _F32, at), _array("state", state, before, tp, at),
         0, _array("lengths", lengths, (b,), _I32, at), _array("d_weight", d_weight, (d, k), _F32, at), _array("d_bias", d_bias, (d,), _F32, at),
         _array("d_final_state", d_final_state, before, tp, at), _array("d_state", d_state, before, tp, at))
     work, address, size = _workspace("myea_b200_causal_convolution_backward_workspace", s, x)
@@ -179,7 +191,7 @@ def _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths):
         raise ValueError("u is [batch, time, width], A [width, states], B and C [batch, time, groups, states]")
     (b, t, d), n, g, tp, at = u.shape, A.shape[1], B.shape[2], u.dtype, u.get_device()
     whole, narrow = (b, t, d), (b, t, g, n)
-    views = _view("u", u, whole, tp, at) + _view("delta", delta, whole, tp, at) + _view("B", B, narrow, tp, at) + _view("C", C_, narrow, tp, at) + _view("z", z, whole, tp, at)
+    views = _own_view("u", u) + _view("delta", delta, whole, tp, at) + _view("B", B, narrow, tp, at) + _view("C", C_, narrow, tp, at) + _view("z", z, whole, tp, at)
     arrays = (_array("A", A, (d, n), _F32, at), _array("D", D, (d,), _F32, at), _array("delta_bias", delta_bias, (d,), _F32, at),
               _array("state", state, (b, d, n), _F32, at))
     return kind, (b, t, d, n, g), at, views, arrays, _array("lengths", lengths, (b,), _I32, at)
@@ -193,12 +205,11 @@ def selective_scan(u, delta, A, B, C_, D=None, z=None, delta_bias=None, softplus
     end, and the state there stays.  checkpoints (scan_checkpoints): kept for selective_scan_backward.  A single token is
     time = 1 with both states."""
     kind, (b, t, d, n, g), at, views, arrays, lengths_at = _scan_inputs(u, delta, A, B, C_, D, z, delta_bias, state, lengths)
-    if out is None:
-        out = _empty_like(u)
+    out, to = _output("out", out, u)
     if final_state is None:
         final_state = u.new_empty((b, d, n), dtype=_F32) if state is None else torch.empty_like(state)
     kept = 0 if checkpoints is None else _array("checkpoints", checkpoints, _checkpoint_shape(b, t, d, n), _F32, at)
-    s = _SCAN.pack(kind, 1 if softplus else 0, 0, 0, b, t, d, n, g, *views, *_view("out", out, (b, t, d), u.dtype, at), *arrays,
+    s = _SCAN.pack(kind, 1 if softplus else 0, 0, 0, b, t, d, n, g, *views, *to, *arrays,
                    _array("final_state", final_state, (b, d, n), _F32, at), lengths_at, kept, *_NO_GRADIENTS)
     work, address, size = _workspace("myea_b200_selective_scan_workspace", s, u)
     _call("myea_b200_selective_scan", at, s, address, size)
@@ -230,12 +241,17 @@ def selective_scan_backward(dy, u, delta, A, B, C_, checkpoints, D=None, z=None,
     return got
 
 
-def _rows(name, x, shape, dtype, index, history=False):
-    """address and row pitch of a [rows, columns] tensor; history: autograd may follow it"""
+def _rows(name, x, shape, dtype, index):
+    """address and row pitch of a [rows, columns] tensor"""
     if x is None:
         return 0, 0
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index:
         _mismatch(name, x, shape, dtype, index)
+    return _own_rows(name, x)
+
+
+def _own_rows(name, x, history=False):
+    """the same for the tensor that the others are compared with; history: autograd may follow it"""
     if not history and x.requires_grad and torch.is_grad_enabled():
         _no_history(name)
     if not x.is_contiguous() and not _dense(x, 1):
@@ -259,7 +275,7 @@ def distillation_error(logits, index, teacher, temperature=1.0, soft=1.0, hard=0
     elif d_logits is None:
         d_logits = _empty_like(logits)
     _call("myea_b200_distillation_error", at, _DISTILLATION.pack(
-        kind, 0, r, v, k, *_rows("logits", logits, (r, v), tp, at), *_rows("index", index, (r, k), _I32, at), *_rows("teacher", teacher, (r, k), _F32, at),
+        kind, 0, r, v, k, *_own_rows("logits", logits), *_rows("index", index, (r, k), _I32, at), *_rows("teacher", teacher, (r, k), _F32, at),
         _array("labels", labels, (r,), _I32, at), _array("weight", weight, (r,), _F32, at), temperature, soft, hard, 0.0,
         _array("losses", losses, (r,), _F32, at), *_rows("d_logits", d_logits, (r, v), tp, at)))
     return losses, d_logits
@@ -280,7 +296,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     if chances is None:
         chances = torch.empty_like(uniform) if uniform is not None else logits.new_empty(one, dtype=_F32)
     _call("myea_b200_sample", at, _SAMPLING.pack(
-        kind, 0, r, v, *_rows("logits", logits, (r, v), logits.dtype, at, True), _array("uniform", uniform, one, _F32, at), _array("temperature", temperature, one, _F32, at),
+        kind, 0, r, v, *_own_rows("logits", logits, True), _array("uniform", uniform, one, _F32, at), _array("temperature", temperature, one, _F32, at),
         _array("top_k", top_k, one, _I32, at), _array("top_p", top_p, one, _F32, at), _array("min_p", min_p, one, _F32, at),
         _array("tokens", tokens, one, _I32, at), _array("chances", chances, one, _F32, at)))
     return tokens, chances
